@@ -392,6 +392,57 @@ int atlb_flow_rk4_bwd(const float* gy, const float* theta, int64_t B, int64_t Hg
 int atlb_rng_uniform2(uint64_t seed, uint64_t call, int64_t n, float* out, atlb_stream_t stream);
 int atlb_rng_normal2(uint64_t seed, uint64_t call, int64_t n, float* out, atlb_stream_t stream);
 
+/* ----------------------------------------------------------------------------------------------
+ * Event-sequence operators: the front of a model whose input is the packed events themselves (one row of D
+ * features per event) and whose output the objectives score.  No counterpart in the reference's ops.
+ * Element types (dtype): ATLB_F32, ATLB_BF16, ATLB_F16; all arrays of one call marked `void*` have that type.  Rows
+ * are contiguous; the row stride ld* (in elements, >= 0) of an input may differ from D, outputs have stride D.
+ * Sums, states and products are fp32, and every output is rounded once.  D <= ATLB_SEQ_MAX_D.
+ * ---------------------------------------------------------------------------------------------- */
+enum { ATLB_F32 = 0, ATLB_BF16 = 1, ATLB_F16 = 2 };
+#define ATLB_SEQ_MAX_D (1 << 20)
+
+/* Row lookup: out[n, :] = scale * weight[idx[n], :], zero where idx[n] lies outside [0, V) (as the gather reads zero
+ * outside the image).  weight (V, D) with row stride ldw, idx (N), out (N, D). */
+int atlb_embedding_fwd(int dtype, const void* weight, int64_t ldw, int64_t V, int64_t D, const int64_t* idx, int64_t N,
+                       double scale, void* out, atlb_stream_t stream);
+/* Its gradient: grad[v, :] = scale * sum over n with idx[n] = v of g[n, :], overwritten (rows no event reads get 0).
+ * The row numbers are sorted and every run summed in the order of its events, in fp32, without atomics: the same
+ * inputs give the same bits.  N < 2^31, V < 2^31 - 1. */
+size_t atlb_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D);
+int atlb_embedding_bwd(int dtype, const void* g, int64_t ldg, const int64_t* idx, int64_t N, int64_t V, int64_t D,
+                       double scale, void* grad, void* workspace, size_t workspace_bytes, atlb_stream_t stream);
+
+/* Dropout whose mask is a function of (seed, call) and is not stored: element i is kept when word i % 4 of
+ * Philox4x32-10 with counter (i / 4, 2^31 | (i / 4) >> 32, call, call >> 32) and key seed is at least
+ * floor(p 2^32 + 1/2); out_i = kept ? x_i / (1 - p) : 0, plus residual_i when residual is not NULL.  The backward
+ * pass is the same call on the incoming gradient, without a residual.  A dropped element is zero whatever x holds.
+ * call_dev: NULL, or one device integer added to call when the kernel runs (a captured graph can draw anew on each
+ * replay).  0 <= p <= 1.  n elements; out must not overlap x or residual. */
+int atlb_dropout(int dtype, const void* x, const void* residual, int64_t n, double p, uint64_t seed, uint64_t call,
+                 const int64_t* call_dev, void* out, atlb_stream_t stream);
+
+/* Gated linear recurrence over the rows of packed windows, per column:
+ *   ATLB_REC_DECAY    h_t = gate_t h_(t-1) + x_t
+ *   ATLB_REC_SIGMOID  h_t = a_t h_(t-1) + (1 - a_t) x_t,  a_t = 1 / (1 + exp(-gate_t))
+ * gate, x (N, D); b (N) the window of each row, the rows of a window contiguous (events sorted by (b, t) are); rows
+ * with b outside [0, B) get h = 0 and no gradient.  b NULL: B equal windows of N / B rows (N a multiple of B).
+ * h0 (B, D) fp32: the state before each window's first row, NULL for zero.  h (N, D); hT (B, D) fp32 or NULL: the
+ * state after each window's last row (h0 for a window without rows).  saved: NULL, or
+ * atlb_recurrence_saved_bytes(N, D) bytes that the backward pass takes. */
+enum { ATLB_REC_DECAY = 0, ATLB_REC_SIGMOID = 1 };
+size_t atlb_recurrence_workspace_bytes(int64_t N, int64_t D);
+size_t atlb_recurrence_saved_bytes(int64_t N, int64_t D);
+int atlb_recurrence_fwd(int dtype, int kind, const void* gate, int64_t ldgate, const void* x, int64_t ldx,
+                        const int64_t* b, int64_t N, int64_t B, int64_t D, const float* h0, void* h, float* hT,
+                        float* saved, void* workspace, size_t workspace_bytes, atlb_stream_t stream);
+/* Its gradient for gh = dL/dh (N, D) and ghT = dL/dhT (B, D), which may be NULL for zero: ggate, gx (N, D), and
+ * gh0 (B, D) unless NULL.  saved: as the forward call of the same inputs left it. */
+int atlb_recurrence_bwd(int dtype, int kind, const void* gate, int64_t ldgate, const void* x, int64_t ldx,
+                        const int64_t* b, int64_t N, int64_t B, int64_t D, const float* h0, const float* saved,
+                        const void* gh, int64_t ldgh, const float* ghT, void* ggate, void* gx, float* gh0,
+                        void* workspace, size_t workspace_bytes, atlb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

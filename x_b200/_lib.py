@@ -116,7 +116,21 @@ _SIGS = {
                                    _size, _vp, _vp, _vp, _vp, _vp]),
     "atlb_exact_prepare_forward": (_int, [ctypes.POINTER(ExactCfg), _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp,
                                           _vp, _vp, _vp, ctypes.POINTER(PlanGeom), _vp, _size, _vp, _vp, _vp, _vp]),
+    "atlb_embedding_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "atlb_embedding_fwd": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, _dbl, _vp, _vp]),
+    "atlb_embedding_bwd": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _i64, _dbl, _vp, _vp, _size, _vp]),
+    "atlb_dropout": (_int, [_int, _vp, _vp, _i64, _dbl, ctypes.c_uint64, ctypes.c_uint64, _vp, _vp, _vp]),
+    "atlb_recurrence_workspace_bytes": (_size, [_i64, _i64]),
+    "atlb_recurrence_saved_bytes": (_size, [_i64, _i64]),
+    "atlb_recurrence_fwd": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
+                                   _size, _vp]),
+    "atlb_recurrence_bwd": (_int, [_int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp,
+                                   _vp, _vp, _vp, _vp, _size, _vp]),
 }
+
+# element types of the event-sequence operators (atlb_dtype of the header)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+REC_KINDS = {"decay": 0, "sigmoid": 1}
 
 _LIB = None
 

@@ -121,6 +121,21 @@ int exact_forward(const atlb_exact_cfg&, const float*, const long long*, long lo
 int exact_backward(const atlb_exact_cfg&, const float*, const long long*, long long, long long, const float*,
                    const atlb_plan_geom&, void*, const float*, const float*, float*, float*, cudaStream_t);
 
+int dropout(int dtype, const void*, const void*, long long, double, unsigned long long, unsigned long long,
+            const long long*, void*, cudaStream_t);
+size_t embedding_workspace_bytes(long long N, long long V, long long D);
+int embedding_fwd(int dtype, const void*, long long, long long, long long, const long long*, long long, double, void*,
+                  cudaStream_t);
+int embedding_bwd(int dtype, const void*, long long, const long long*, long long, long long, long long, double, void*,
+                  void*, cudaStream_t);
+size_t recurrence_workspace_bytes(long long N, long long D);
+size_t recurrence_saved_bytes(long long N, long long D);
+int recurrence_fwd(int dtype, int kind, const void*, long long, const void*, long long, const long long*, long long,
+                   long long, long long, const float*, void*, float*, float*, void*, cudaStream_t);
+int recurrence_bwd(int dtype, int kind, const void*, long long, const void*, long long, const long long*, long long,
+                   long long, long long, const float*, const float*, const void*, long long, const float*, void*,
+                   void*, float*, void*, cudaStream_t);
+
 }  // namespace atlb
 
 using namespace atlb;
@@ -619,6 +634,115 @@ int atlb_exact_backward(const atlb_exact_cfg* cfg, const float* grad_ls, const i
     return ATLB_ERR_WORKSPACE;
   }
   return exact_backward(*cfg, grad_ls, LL(b), N, M, ev4, *geom, workspace, S, den, gv, gtheta, STREAM(stream));
+}
+
+// ---------------------------------------------------------------------------------------------- event-sequence ops
+static int check_seq(int dtype, int64_t N, int64_t D, const char* fn) {
+  if (dtype != ATLB_F32 && dtype != ATLB_BF16 && dtype != ATLB_F16) {
+    set_error("%s: unknown dtype %d", fn, dtype);
+    return ATLB_ERR_ARG;
+  }
+  if (N > (1LL << 31) - 1 || D > ATLB_SEQ_MAX_D) {
+    set_error("%s: %lld rows of %lld columns exceed the kernels' sizes", fn, (long long)N, (long long)D);
+    return ATLB_ERR_OVERFLOW;
+  }
+  return ATLB_OK;
+}
+
+static int check_ws(const void* ws, size_t have, size_t need, const char* fn) {
+  if (!ws || have < need) {
+    set_error("%s: workspace %zu < %zu bytes", fn, have, need);
+    return ATLB_ERR_WORKSPACE;
+  }
+  return ATLB_OK;
+}
+
+size_t atlb_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D) {
+  return embedding_workspace_bytes(N < 0 ? 0 : N, V < 0 ? 0 : V, D < 0 ? 0 : D);
+}
+
+static int check_rows(int64_t V, const char* fn) {
+  if (V >= (1LL << 31) - 1) {
+    set_error("%s: %lld table rows exceed the 32-bit row numbers", fn, (long long)V);
+    return ATLB_ERR_OVERFLOW;
+  }
+  return ATLB_OK;
+}
+
+int atlb_embedding_fwd(int dtype, const void* weight, int64_t ldw, int64_t V, int64_t D, const int64_t* idx, int64_t N,
+                       double scale, void* out, atlb_stream_t stream) {
+  clear();
+  NONNEG(N); NONNEG(V); NONNEG(D); NONNEG(ldw);
+  if (int st = check_seq(dtype, N, D, __func__)) return st;
+  if (int st = check_rows(V, __func__)) return st;
+  NEED(weight, V * D); NEED(idx, N); NEED(out, N * D);
+  return embedding_fwd(dtype, weight, ldw, V, D, LL(idx), N, scale, out, STREAM(stream));
+}
+
+int atlb_embedding_bwd(int dtype, const void* g, int64_t ldg, const int64_t* idx, int64_t N, int64_t V, int64_t D,
+                       double scale, void* grad, void* workspace, size_t workspace_bytes, atlb_stream_t stream) {
+  clear();
+  NONNEG(N); NONNEG(V); NONNEG(D); NONNEG(ldg);
+  if (int st = check_seq(dtype, N, D, __func__)) return st;
+  if (int st = check_rows(V, __func__)) return st;
+  NEED(g, N * D); NEED(idx, N); NEED(grad, V * D);
+  if (int st = check_ws(workspace, workspace_bytes, embedding_workspace_bytes(N, V, D), __func__)) return st;
+  return embedding_bwd(dtype, g, ldg, LL(idx), N, V, D, scale, grad, workspace, STREAM(stream));
+}
+
+int atlb_dropout(int dtype, const void* x, const void* residual, int64_t n, double p, uint64_t seed, uint64_t call,
+                 const int64_t* call_dev, void* out, atlb_stream_t stream) {
+  clear();
+  NONNEG(n);
+  if (int st = check_seq(dtype, 0, 0, __func__)) return st;
+  if (!(p >= 0.0 && p <= 1.0)) { set_error("%s: p = %g lies outside [0, 1]", __func__, p); return ATLB_ERR_ARG; }
+  NEED(x, n); NEED(out, n);
+  return dropout(dtype, x, residual, n, p, seed, call, LL(call_dev), out, STREAM(stream));
+}
+
+size_t atlb_recurrence_workspace_bytes(int64_t N, int64_t D) {
+  return recurrence_workspace_bytes(N < 0 ? 0 : N, D < 0 ? 0 : D);
+}
+size_t atlb_recurrence_saved_bytes(int64_t N, int64_t D) {
+  return recurrence_saved_bytes(N < 0 ? 0 : N, D < 0 ? 0 : D);
+}
+
+static int check_rec(int dtype, int kind, const int64_t* b, int64_t N, int64_t B, int64_t D, const char* fn) {
+  if (int st = check_seq(dtype, N, D, fn)) return st;
+  if (kind != ATLB_REC_DECAY && kind != ATLB_REC_SIGMOID) {
+    set_error("%s: unknown recurrence kind %d", fn, kind);
+    return ATLB_ERR_ARG;
+  }
+  if (B > (1LL << 31) - 1) { set_error("%s: too many windows", fn); return ATLB_ERR_OVERFLOW; }
+  if (!b && N > 0 && (B < 1 || N % B != 0)) {
+    set_error("%s: %lld rows do not make %lld equal windows", fn, (long long)N, (long long)B);
+    return ATLB_ERR_ARG;
+  }
+  return ATLB_OK;
+}
+
+int atlb_recurrence_fwd(int dtype, int kind, const void* gate, int64_t ldgate, const void* x, int64_t ldx,
+                        const int64_t* b, int64_t N, int64_t B, int64_t D, const float* h0, void* h, float* hT,
+                        float* saved, void* workspace, size_t workspace_bytes, atlb_stream_t stream) {
+  clear();
+  NONNEG(N); NONNEG(B); NONNEG(D); NONNEG(ldgate); NONNEG(ldx);
+  if (int st = check_rec(dtype, kind, b, N, B, D, __func__)) return st;
+  NEED(gate, N * D); NEED(x, N * D); NEED(h, N * D);
+  if (int st = check_ws(workspace, workspace_bytes, recurrence_workspace_bytes(N, D), __func__)) return st;
+  return recurrence_fwd(dtype, kind, gate, ldgate, x, ldx, LL(b), N, B, D, h0, h, hT, saved, workspace, STREAM(stream));
+}
+
+int atlb_recurrence_bwd(int dtype, int kind, const void* gate, int64_t ldgate, const void* x, int64_t ldx,
+                        const int64_t* b, int64_t N, int64_t B, int64_t D, const float* h0, const float* saved,
+                        const void* gh, int64_t ldgh, const float* ghT, void* ggate, void* gx, float* gh0,
+                        void* workspace, size_t workspace_bytes, atlb_stream_t stream) {
+  clear();
+  NONNEG(N); NONNEG(B); NONNEG(D); NONNEG(ldgate); NONNEG(ldx); NONNEG(ldgh);
+  if (int st = check_rec(dtype, kind, b, N, B, D, __func__)) return st;
+  NEED(gate, N * D); NEED(x, N * D); NEED(gh, N * D); NEED(ggate, N * D); NEED(gx, N * D); NEED(saved, N * D);
+  if (int st = check_ws(workspace, workspace_bytes, recurrence_workspace_bytes(N, D), __func__)) return st;
+  return recurrence_bwd(dtype, kind, gate, ldgate, x, ldx, LL(b), N, B, D, h0, saved, gh, ldgh, ghT, ggate, gx, gh0,
+                        workspace, STREAM(stream));
 }
 
 }  // extern "C"

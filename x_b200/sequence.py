@@ -1,0 +1,268 @@
+"""Event-sequence operators: the front of a model whose input is the packed events themselves.
+
+The objectives score a motion; a model that produces it from events needs, per event, a row of features
+(:func:`embedding`), regularisation while it trains (:func:`dropout`) and a state that runs along each window's
+events (:func:`linear_recurrence`).  All three work on the layout of the other ops of this package: one row per event,
+windows packed one behind the other and sorted by (b, t), ``b`` (N,) int64.  The reference's ops have no counterpart.
+
+float32, bfloat16 and float16; sums, states and products are held in float32 and every output is rounded once.  The
+kernels run on the tensors' device and its current stream, allocate with torch and never synchronise, so calls can be
+captured in CUDA graphs; a backward pass only while no eager autograd graph of the same leaves lives (torch ties a
+leaf's gradient to the stream of its first graph, and the capture fails).  Results do not depend on the timing of a
+run.  There is no CPU path, and the gradients are not differentiable again.
+"""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+
+_MASK64 = 2**64 - 1
+
+
+# ------------------------------------------------------------------------------------------- arguments
+def _need(what: str, **tensors):
+    """Every given tensor on one CUDA device; the first decides."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"x_b200.{what}: {name} must be a CUDA tensor (there is no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"x_b200.{what}: {name} lies on {t.device}, the other tensors on {dev}")
+    return dev
+
+
+def _need_dtype(what: str, name: str, t, dtypes):
+    if t is not None and t.dtype not in dtypes:
+        raise RuntimeError(f"x_b200.{what}: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+
+
+def _on(dev):
+    """The device of the tensors for the launch, if it is not the current one."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _rows(t):
+    """(t, row stride) with neighbouring elements in each row of the 2-D tensor; a copy where they are not."""
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------------------------------------------- embedding
+def _embedding_fwd(weight, idx, scale):
+    w, ldw = _rows(weight)
+    V, D = w.shape
+    with _on(w.device):
+        out = torch.empty(*idx.shape, D, dtype=w.dtype, device=w.device)
+        L.check(L.lib().atlb_embedding_fwd(L.DTYPES[w.dtype], w.data_ptr(), ldw, V, D, idx.data_ptr(), idx.numel(),
+                                           scale, out.data_ptr(), L.stream()), "embedding")
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, idx, scale):
+        ctx.save_for_backward(idx)
+        ctx.meta = (weight.shape, scale)
+        return _embedding_fwd(weight, idx, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (idx,) = ctx.saved_tensors
+        (V, D), scale = ctx.meta
+        g, ldg = _rows(g.reshape(idx.numel(), D))
+        N = idx.numel()
+        lib = L.lib()
+        with _on(g.device):
+            grad = torch.empty(V, D, dtype=g.dtype, device=g.device)
+            nb = lib.atlb_embedding_workspace_bytes(N, V, D)
+            ws = L.workspace(nb, g.device)
+            L.check(lib.atlb_embedding_bwd(L.DTYPES[g.dtype], g.data_ptr(), ldg, idx.data_ptr(), N, V, D, scale,
+                                           grad.data_ptr(), ws.data_ptr(), nb, L.stream()), "embedding_bwd")
+        return grad, None, None
+
+
+def embedding(weight: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """Rows of a table, scaled: ``scale * weight[idx]``, of shape ``idx.shape + (D,)``.
+
+    weight (V, D) float32, bfloat16 or float16; idx integers of any shape.  An index outside [0, V) reads a row of
+    zeros and gives no gradient, as :func:`x_b200.gather` does outside the image: events that left the sensor and
+    padding (-1) need no mask.  The gradient of ``weight`` is summed over the events of each row in their order, in
+    float32 and without atomics; rows that no event reads get zeros."""
+    _need("embedding", weight=weight, idx=idx)
+    if weight.dim() != 2:
+        raise ValueError(f"x_b200.embedding: weight must be (V, D), got {tuple(weight.shape)}")
+    _need_dtype("embedding", "weight", weight, L.DTYPES)
+    _need_dtype("embedding", "idx", idx, (torch.int64, torch.int32, torch.int16, torch.uint8))
+    idx = idx.long().contiguous()
+    if _wants_grad(weight):
+        return _Embedding.apply(weight, idx, float(scale))
+    return _embedding_fwd(weight, idx, float(scale))
+
+
+# ------------------------------------------------------------------------------------------- dropout
+def _dropout_run(x, residual, p, seed, call):
+    x = x.contiguous()
+    dev_call = call if torch.is_tensor(call) else None
+    with _on(x.device):
+        out = torch.empty_like(x)
+        L.check(L.lib().atlb_dropout(L.DTYPES[x.dtype], x.data_ptr(), _addr(residual), x.numel(), p, seed,
+                                     0 if dev_call is not None else call, _addr(dev_call), out.data_ptr(),
+                                     L.stream()), "dropout")
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, call):
+        ctx.meta = (p, seed, None if torch.is_tensor(call) else call)
+        ctx.save_for_backward(*([call] if torch.is_tensor(call) else []))
+        return _dropout_run(x, residual, p, seed, call)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        p, seed, call = ctx.meta
+        if call is None:
+            (call,) = ctx.saved_tensors
+        gx = _dropout_run(g, None, p, seed, call) if ctx.needs_input_grad[0] else None
+        return gx, g if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, call=0, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """Dropout from the counter-based generator of :mod:`x_b200.rng`: each element of x is kept with probability
+    1 - p and scaled by 1 / (1 - p), or becomes 0 whatever it held.  With ``residual`` (shape and dtype of x) the
+    result is ``residual + dropout(x)``, rounded once.
+
+    The mask is a function of (seed, call) and the element's index and is never stored: the backward pass draws it
+    again.  Give every place and step that drops its own (seed, call), for instance
+    ``dropout(x, p, draws.seed, draws.next_call())`` with a :class:`x_b200.rng.DeviceDraws`; the same pair gives the
+    same mask.  ``call`` may be a one-element int64 tensor on x's device instead, read when the kernel runs: a captured
+    CUDA graph that adds to it after its backward pass drops anew on every replay."""
+    dev = _need("dropout", x=x, residual=residual)
+    _need_dtype("dropout", "x", x, L.DTYPES)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"x_b200.dropout: p = {p} lies outside [0, 1]")
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"x_b200.dropout: residual is {tuple(residual.shape)} {residual.dtype}, "
+                             f"x {tuple(x.shape)} {x.dtype}")
+        residual = residual.contiguous()
+    if torch.is_tensor(call):
+        if call.numel() != 1 or call.dtype != torch.int64 or call.device != dev:
+            raise ValueError("x_b200.dropout: call must be an integer or a one-element int64 tensor on x's device")
+    else:
+        call = int(call) & _MASK64
+    seed = int(seed) & _MASK64
+    if _wants_grad(x, residual):
+        return _Dropout.apply(x, residual, float(p), seed, call)
+    return _dropout_run(x, residual, float(p), seed, call)
+
+
+# ------------------------------------------------------------------------------------------- recurrence
+def _recurrence_fwd(gate, x, b, B, h0, kind, want_state, save):
+    gate, ldgate = _rows(gate)
+    x, ldx = _rows(x)
+    N, D = x.shape
+    dev, lib = x.device, L.lib()
+    with _on(dev):
+        h = torch.empty(N, D, dtype=x.dtype, device=dev)
+        hT = torch.empty(B, D, dtype=torch.float32, device=dev) if want_state else None
+        saved = L.workspace(lib.atlb_recurrence_saved_bytes(N, D), dev) if save else None
+        nb = lib.atlb_recurrence_workspace_bytes(N, D)
+        ws = L.workspace(nb, dev)
+        L.check(lib.atlb_recurrence_fwd(L.DTYPES[x.dtype], kind, gate.data_ptr(), ldgate, x.data_ptr(), ldx, _addr(b),
+                                        N, B, D, _addr(h0), h.data_ptr(), _addr(hT), _addr(saved), ws.data_ptr(), nb,
+                                        L.stream()), "linear_recurrence")
+    return h, hT, saved
+
+
+class _Recurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, x, b, B, h0, kind, want_state):
+        h, hT, saved = _recurrence_fwd(gate, x, b, B, h0, kind, want_state, True)
+        ctx.save_for_backward(gate, x, b, h0, saved)
+        ctx.meta = (B, kind)
+        ctx.set_materialize_grads(False)
+        return h, hT
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gh, ghT):
+        gate, x, b, h0, saved = ctx.saved_tensors
+        B, kind = ctx.meta
+        gate, ldgate = _rows(gate)
+        x, ldx = _rows(x)
+        gh, ldgh = _rows(torch.zeros_like(x) if gh is None else gh)
+        ghT = None if ghT is None else ghT.contiguous()
+        N, D = x.shape
+        dev, lib = x.device, L.lib()
+        with _on(dev):
+            ggate, gx = (torch.empty(N, D, dtype=x.dtype, device=dev) for _ in range(2))
+            gh0 = torch.empty(B, D, dtype=torch.float32, device=dev) if h0 is not None else None
+            nb = lib.atlb_recurrence_workspace_bytes(N, D)
+            ws = L.workspace(nb, dev)
+            L.check(lib.atlb_recurrence_bwd(L.DTYPES[x.dtype], kind, gate.data_ptr(), ldgate, x.data_ptr(), ldx,
+                                            _addr(b), N, B, D, _addr(h0), saved.data_ptr(), gh.data_ptr(), ldgh,
+                                            _addr(ghT), ggate.data_ptr(), gx.data_ptr(), _addr(gh0), ws.data_ptr(), nb,
+                                            L.stream()), "linear_recurrence_bwd")
+        return ggate, gx, None, None, gh0, None, None
+
+
+def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, b: torch.Tensor | None = None, B: int = 1,
+                      h0: torch.Tensor | None = None, kind: str = "sigmoid", return_state: bool = False):
+    """A state per column that runs along the rows of each window:
+
+        kind="sigmoid"  h_t = a_t h_(t-1) + (1 - a_t) x_t,  a_t = sigmoid(gate_t)
+        kind="decay"    h_t = gate_t h_(t-1) + x_t          (exp(-dt / tau): decaying event traces)
+
+    gate, x (N, D), one dtype; slices of a wider projection are taken as they are.  ``b`` (N,) int64 is the window of
+    each row in [0, B), the rows of a window contiguous, as in events sorted by (b, t); rows with any other value
+    (padding, -1) get h = 0 and no gradient, and what they hold reaches nothing.  Without ``b`` the rows are B equal
+    windows: a (B, T, D) batch is ``flatten(0, 1)``.  ``h0`` (B, D) float32 is the state before each window's first
+    row (default zero).  Returns h (N, D), or (h, state) with ``return_state``: state (B, D) float32 after each
+    window's last row (h0 where a window has none), to be given as the next call's ``h0``; one row per window is one
+    step.  Differentiable in gate, x and h0, through h and state."""
+    _need("linear_recurrence", x=x, gate=gate, b=b, h0=h0)
+    _need_dtype("linear_recurrence", "x", x, L.DTYPES)
+    if x.dim() != 2 or gate.shape != x.shape or gate.dtype != x.dtype:
+        raise ValueError(f"x_b200.linear_recurrence: gate and x must be (N, D) of one dtype, got "
+                         f"{tuple(gate.shape)} {gate.dtype} and {tuple(x.shape)} {x.dtype}")
+    if kind not in L.REC_KINDS:
+        raise ValueError(f"x_b200.linear_recurrence: unknown kind {kind!r}")
+    N, D = x.shape
+    B = int(B)
+    if B < 0 or (b is None and (B < 1 or N % B)):
+        raise ValueError(f"x_b200.linear_recurrence: {N} rows do not make {B} equal windows")
+    if b is not None:
+        _need_dtype("linear_recurrence", "b", b, (torch.int64,))
+        if b.shape != (N,):
+            raise ValueError(f"x_b200.linear_recurrence: b must be ({N},), got {tuple(b.shape)}")
+        b = b.contiguous()
+    if h0 is not None:
+        _need_dtype("linear_recurrence", "h0", h0, (torch.float32,))
+        if h0.shape != (B, D):
+            raise ValueError(f"x_b200.linear_recurrence: h0 must be ({B}, {D}), got {tuple(h0.shape)}")
+        h0 = h0.contiguous()
+    if _wants_grad(gate, x, h0):
+        h, state = _Recurrence.apply(gate, x, b, B, h0, L.REC_KINDS[kind], return_state)
+    else:
+        h, state, _ = _recurrence_fwd(gate, x, b, B, h0, L.REC_KINDS[kind], return_state, False)
+    return (h, state) if return_state else h

@@ -15,7 +15,7 @@ namespace {
 constexpr int kThreads = 256;
 
 struct Drop {
-  unsigned k0, k1;              // seed words
+  unsigned key[20];             // the ten rounds' keys, so that a round takes them from constant memory
   unsigned long long call;
   const long long* call_dev;    // added to call when not null: a graph replay can draw anew
   unsigned threshold;           // keep when the word is at least this
@@ -23,34 +23,94 @@ struct Drop {
   float scale;
 };
 
-__device__ __forceinline__ Philox4 drop_words(const Drop& D, unsigned long long call, unsigned long long q) {
-  return philox4x32_10(Philox4{(unsigned)q, (unsigned)(q >> 32) | 0x80000000u, (unsigned)call, (unsigned)(call >> 32)},
-                       D.k0, D.k1);
+// The four words of counter q: philox4x32_10 (rng.cuh) with the keys laid out ahead.
+__device__ __forceinline__ void drop_words(const Drop& D, unsigned long long call, unsigned long long q,
+                                           unsigned (&w)[4]) {
+  Philox4 c{(unsigned)q, (unsigned)(q >> 32) | 0x80000000u, (unsigned)call, (unsigned)(call >> 32)};
+#pragma unroll
+  for (int r = 0; r < 10; ++r) c = philox_round(c, D.key[2 * r], D.key[2 * r + 1]);
+  w[0] = c.x, w[1] = c.y, w[2] = c.z, w[3] = c.w;
 }
 
 __device__ __forceinline__ float drop_one(const Drop& D, unsigned word, float x) {
   return (word >= D.threshold && !D.none) ? x * D.scale : 0.f;
 }
 
-// One thread per group of four elements (one Philox call).
+// A vector of 16 bytes is one Philox call of fp32 or two of 16-bit elements.  VECS vectors per thread, their loads
+// issued together: at 64M bf16 elements one pass moves 256 MB in 45 us (5.7 TB/s, 88 % of the copy rate), as fast as
+// with half or twice the vectors; the words cost 40 instructions per four elements and hide under it.  Element by
+// element, where a pointer is not on a 16-byte boundary, it takes 95 us.
+template <typename T, bool RES, int VECS>
+__global__ void __launch_bounds__(kThreads) k_dropout_vec(Drop D, const T* __restrict__ x, const T* __restrict__ res,
+                                                          long long n, T* __restrict__ out) {
+  constexpr int E = 16 / sizeof(T);
+  const unsigned long long call = D.call + (D.call_dev ? (unsigned long long)*D.call_dev : 0ull);
+  const long long vecs = n / E, v0 = blockIdx.x * (long long)(kThreads * VECS) + threadIdx.x;
+  Pack<T, E> xv[VECS], rv[VECS];
+#pragma unroll
+  for (int k = 0; k < VECS; ++k) {
+    const long long v = v0 + k * kThreads;
+    if (v < vecs) {
+      xv[k] = load_pack<T, E>(x + v * E);
+      if (RES) rv[k] = load_pack<T, E>(res + v * E);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VECS; ++k) {
+    const long long v = v0 + k * kThreads;
+    if (v < vecs) {
+#pragma unroll
+      for (int g = 0; g < E / 4; ++g) {
+        unsigned w[4];
+        drop_words(D, call, (unsigned long long)v * (E / 4) + g, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y = drop_one(D, w[j], to_f32(xv[k].v[g * 4 + j]));
+          if (RES) y += to_f32(rv[k].v[g * 4 + j]);
+          xv[k].v[g * 4 + j] = from_f32<T>(y);
+        }
+      }
+      store_pack(out + v * E, xv[k]);
+    }
+  }
+}
+
+// Elements from `from` on, four (one Philox call) per thread.
 template <typename T, bool RES>
 __global__ void __launch_bounds__(kThreads) k_dropout(Drop D, const T* __restrict__ x, const T* __restrict__ res,
-                                                      long long n, T* __restrict__ out) {
+                                                      long long from, long long n, T* __restrict__ out) {
   const unsigned long long call = D.call + (D.call_dev ? (unsigned long long)*D.call_dev : 0ull);
   const long long groups = (n + 3) / 4, stride = (long long)gridDim.x * blockDim.x;
-  for (long long q = blockIdx.x * (long long)blockDim.x + threadIdx.x; q < groups; q += stride) {
-    const Philox4 w = drop_words(D, call, (unsigned long long)q);
-    const unsigned word[4] = {w.x, w.y, w.z, w.w};
+  for (long long q = from / 4 + blockIdx.x * (long long)blockDim.x + threadIdx.x; q < groups; q += stride) {
+    unsigned w[4];
+    drop_words(D, call, (unsigned long long)q, w);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const long long i = q * 4 + j;
       if (i < n) {
-        float v = drop_one(D, word[j], to_f32(x[i]));
-        if (RES) v += to_f32(res[i]);
-        out[i] = from_f32<T>(v);
+        float y = drop_one(D, w[j], to_f32(x[i]));
+        if (RES) y += to_f32(res[i]);
+        out[i] = from_f32<T>(y);
       }
     }
   }
+}
+
+template <typename T, bool RES>
+int run(const Drop& D, const T* x, const T* res, long long n, T* out, cudaStream_t s) {
+  constexpr int E = 16 / sizeof(T), VECS = 2;
+  long long done = 0;
+  if (aligned_to(x, 16) && aligned_to(out, 16) && (!RES || aligned_to(res, 16))) {
+    const long long vecs = n / E, per = kThreads * VECS;
+    if (vecs > 0)
+      launch(k_dropout_vec<T, RES, VECS>, (unsigned)((vecs + per - 1) / per), kThreads, 0, s, D, x, res, n, out);
+    done = vecs * E;
+  }
+  if (done < n) {  // the rest, fewer than E elements behind whole vectors
+    const int grid = clamp_grid(((n - done + 3) / 4 + kThreads - 1) / kThreads);
+    launch(k_dropout<T, RES>, grid, kThreads, 0, s, D, x, res, done, n, out);
+  }
+  return launch_status("dropout");
 }
 
 }  // namespace
@@ -59,16 +119,17 @@ int dropout(int dtype, const void* x, const void* residual, long long n, double 
             unsigned long long call, const long long* call_dev, void* out, cudaStream_t s) {
   if (n <= 0) return ATLB_OK;
   const unsigned long long t = (unsigned long long)(p * 4294967296.0 + 0.5);
-  Drop D{(unsigned)seed, (unsigned)(seed >> 32), call, call_dev, (unsigned)t, t > 0xffffffffull,
-         p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f};
+  Drop D;
+  philox_keys((unsigned)seed, (unsigned)(seed >> 32), D.key);
+  D.call = call;
+  D.call_dev = call_dev;
+  D.threshold = (unsigned)t;
+  D.none = t > 0xffffffffull;
+  D.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
   return with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
-    const int grid = clamp_grid((n / 4 + kThreads) / kThreads);
-    if (residual)
-      launch(k_dropout<T, true>, grid, kThreads, 0, s, D, (const T*)x, (const T*)residual, n, (T*)out);
-    else
-      launch(k_dropout<T, false>, grid, kThreads, 0, s, D, (const T*)x, (const T*)nullptr, n, (T*)out);
-    return launch_status("dropout");
+    if (residual) return run<T, true>(D, (const T*)x, (const T*)residual, n, (T*)out, s);
+    return run<T, false>(D, (const T*)x, nullptr, n, (T*)out, s);
   });
 }
 

@@ -7,399 +7,431 @@
 //   decay    dgate = g_t h_(t-1)                          dx = g_t
 //   sigmoid  dgate = g_t (h_(t-1) - x_t) a_t (1 - a_t)    dx = (1 - a_t) g_t
 //
-// Rows are cut into chunks of kRows; over a chunk the recurrence is an affine map h -> A h + C of the state that
-// enters it (and u -> A u + C' backward, with the same A), so the chunks' maps are found side by side, chained, and
-// the rows then replayed from their true state.  States, maps and sums are fp32; an output is rounded once.  A row
-// that begins a window drops what comes before it by selection, so nothing of one window, NaN included, reaches
-// another.
+// Rows are cut into groups of kGroup; over a group the recurrence is an affine map h -> A h + C of the state that enters
+// it (and u -> A u + C' backward, with the same A).  Three kernels: the maps of the groups, joined inside each CTA's
+// chunk of groups (k_rec_map); the states between the chunks (k_rec_chain); the rows replayed from the true state of
+// their group (k_rec_fwd, k_rec_bwd).  Inputs are read twice and nothing waits for another CTA: a single pass, with
+// tiles in shared memory that post their maps to one another, reads them once but measured 647 us where this one
+// takes 425 us (forward and backward, 1M rows of 64 bf16 columns), the waits and the link costing more than the bytes.
+// The maps are joined in one fixed order.  States, maps and sums are fp32; an output is rounded once.  A row that
+// begins a window drops what comes before it by selection, so nothing of one window, NaN included, reaches another.
 #include "vec.cuh"
 
 namespace atlb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kWarpRows = 16;                 // rows of one warp
-constexpr int kRows = kWarps * kWarpRows;     // rows of one chunk
+constexpr int kGroup = 32;          // rows of a group
+constexpr int kPart = 8;                      // rows between the states that the forward pass keeps for the backward pass
+constexpr int kBytes = 8;           // of a row per thread, where the rows are whole multiples of it
+constexpr int kSeg = 16;            // groups joined by one thread
+constexpr int kChainCols = 8, kChainSegs = 128;
 
 struct RecShape {
-  long long N, T;          // rows; rows per window where b is null
+  long long N;             // rows, below 2^31
+  unsigned T;              // rows per window where b is null
   int B, D;
   const long long* b;      // window of every row, or null
+  int groups, chunks;      // groups of rows, chunks of groups
+  int lanes;               // threads per row in k_rec_map and k_rec_fwd (a power of two)
+  bool linked;             // false: every group begins a window, no state enters one
 };
 
-// Windows of a warp's rows: bit i of `first` / `last` marks row i as the first / last of its window, `valid` as one
-// that belongs to a window at all; win is the window of row `lane`.
-struct RowFlags {
-  unsigned first, last, valid;
-  int win;
-};
-
-__device__ __forceinline__ RowFlags row_flags(const RecShape& S, long long r0, int lane) {
-  const long long n = r0 + lane;
-  bool first = false, last = false, valid = false;
-  int win = -1;
-  if (lane < kWarpRows && n < S.N) {
-    if (S.b) {
-      const long long w = S.b[n];
-      valid = w >= 0 && w < S.B;
-      first = n == 0 || S.b[n - 1] != w;
-      last = n + 1 == S.N || S.b[n + 1] != w;
-      win = valid ? (int)w : -1;
-    } else {
-      win = (int)(n / S.T);
-      const long long t = n - win * S.T;
-      valid = true;
-      first = t == 0;
-      last = t + 1 == S.T;
-    }
-  }
-  RowFlags f;
-  f.first = __ballot_sync(0xffffffffu, first);
-  f.last = __ballot_sync(0xffffffffu, last);
-  f.valid = __ballot_sync(0xffffffffu, valid);
-  f.win = win;
-  return f;
+// a = 1 / (1 + exp(-z)) and 1 - a = exp(-z) a.  The exponent is capped so that exp(-z) stays finite: below -87 a is
+// held at 2^-126, where fp32's normal numbers end.
+__device__ __forceinline__ void sigmoid2(float z, float* a, float* w) {
+  float e, r;
+  const float t = fminf(z * -1.44269504f, 126.f);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  *a = z == z ? r : z;  // fminf passes a NaN over
+  *w = e * *a;
 }
 
-// a = 1 / (1 + exp(-z)) and 1 - a, each from exp(-|z|), which does not overflow, so neither cancels.
-__device__ __forceinline__ void sigmoid2(float z, float* a, float* na) {
-  const float e = __expf(-fabsf(z));
-  const float r = __fdividef(1.f, 1.f + e), s = e * r;
-  *a = z >= 0.f ? r : s;
-  *na = z >= 0.f ? s : r;
-}
-
+// The row's coefficient a and what it adds: (1 - a) x or x.
 template <int KIND>
-__device__ __forceinline__ void row_coeff(float gate, float* a, float* w) {
+__device__ __forceinline__ void row_terms(float gate, float x, float* a, float* w, float* v) {
   if (KIND == ATLB_REC_SIGMOID) {
     sigmoid2(gate, a, w);
+    *v = *w * x;
   } else {
     *a = gate;
     *w = 1.f;
+    *v = x;
   }
 }
 
-// State after rows whose map is (A, C).  A zero state leaves C: the product of many gates above one may overflow.
-__device__ __forceinline__ float through(float A, float C, float s) { return s == 0.f ? C : fmaf(A, s, C); }
+// ------------------------------------------------------------------------------------------------ maps
+// The map of some rows in one column; cut: they hold a window's border, so the state before them does not matter.
+struct Map {
+  float A, C;
+  bool cut;
+};
+__device__ __forceinline__ Map identity() { return Map{1.f, 0.f, false}; }
+// A zero state leaves C: the product of many gates above one may overflow.
+__device__ __forceinline__ float apply(const Map& m, float s) { return m.cut || s == 0.f ? m.C : fmaf(m.A, s, m.C); }
+__device__ __forceinline__ Map then(const Map& a, const Map& b) { return Map{a.A * b.A, apply(b, a.C), a.cut || b.cut}; }
+
+// As 64 bits: A below, C above; a cut stands in the place of A, as a NaN that arithmetic does not make.
+constexpr unsigned kCut = 0x7fc00c07u, kNan = 0x7fffffffu;
+__device__ __forceinline__ uint2 pack_map(const Map& m) {
+  return make_uint2(m.cut ? kCut : (m.A != m.A ? kNan : __float_as_uint(m.A)), __float_as_uint(m.C));
+}
+__device__ __forceinline__ Map unpack_map(uint2 v) { return Map{__uint_as_float(v.x), __uint_as_float(v.y), v.x == kCut}; }
+
+// ------------------------------------------------------------------------------------------------ windows
+// Bit r of each word stands for row r of the group: `first` / `last` of its window, `none` when it belongs to no window
+// or lies behind the last row.
+struct Edges {
+  unsigned first, last, none;
+};
+
+__device__ __forceinline__ void row_edges(const RecShape& S, long long n, bool* first, bool* last, bool* none) {
+  if (n >= S.N) {
+    *first = *last = false;
+    *none = true;
+  } else if (S.b) {
+    const long long w = S.b[n];
+    *none = w < 0 || w >= S.B;
+    *first = n == 0 || S.b[n - 1] != w;
+    *last = n + 1 == S.N || S.b[n + 1] != w;
+  } else {
+    const unsigned t = (unsigned)n % S.T;
+    *none = false;
+    *first = t == 0;
+    *last = t + 1 == S.T;
+  }
+}
+
+// The edges of this thread's group; a warp holds `per` neighbouring groups from g0 on, the thread's is number mine.
+__device__ __forceinline__ Edges group_edges(const RecShape& S, long long g0, int per, int mine) {
+  Edges e{0, 0, 0};
+  for (int i = 0; i < per; ++i) {
+    bool first, last, none;
+    row_edges(S, (g0 + i) * kGroup + (threadIdx.x & 31), &first, &last, &none);
+    const unsigned f = __ballot_sync(0xffffffffu, first), l = __ballot_sync(0xffffffffu, last),
+                   v = __ballot_sync(0xffffffffu, none);
+    if (i == mine) e = Edges{f, l, v};
+  }
+  return e;
+}
+
+__device__ __forceinline__ int window_of(const RecShape& S, long long n) {
+  return S.b ? (int)S.b[n] : (int)((unsigned)n / S.T);
+}
+
+template <int E>
+__device__ __forceinline__ void load_state(const float* p, long long row, int D, int c, bool in, float (&s)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) s[e] = in && p ? p[row * D + c + e] : 0.f;
+}
 
 template <typename T, int E>
-__device__ __forceinline__ Pack<T, E> load_row(const T* p, long long ld, long long n, int c, bool in) {
+__device__ __forceinline__ Pack<T, E> load_or_zero(const T* p, bool in) {
+  if (in) return load_pack<T, E>(p);
   Pack<T, E> r;
-  if (in) {
-    r = load_pack<T, E>(p + n * ld + c);
-  } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) r.v[e] = from_f32<T>(0.f);
-  }
+  for (int e = 0; e < E; ++e) r.v[e] = from_f32<T>(0.f);
   return r;
 }
 
-// Maps of the chunks, forward (BWD false: C is the state after the chunk from zero) or backward (u before it).
-// map holds A, then C, each (chunks, D); drop[chunk] is set when a window border inside the chunk cuts it off from
-// the state that enters it.
+template <typename T>
+struct Src {
+  const T* p;
+  long long ld;
+};
+
+// ------------------------------------------------------------------------------------------------ maps of the groups
+// Threads `lanes` wide on a row, E neighbouring columns each; the CTA's groups are one chunk.  BWD walks from the last
+// row to the first: in = dL/dh, and the state is u.  prefix: the map from the chunk's entry to the group's; chunk: the
+// whole chunk's map.
+constexpr int kAhead = 4;  // rows in flight per thread
+
 template <typename T, int E, int KIND, bool BWD>
-__global__ void __launch_bounds__(kThreads) k_rec_map(RecShape S, const T* __restrict__ gate, long long ldg,
-                                                      const T* __restrict__ in, long long ldi,
-                                                      const float* __restrict__ h0, const float* __restrict__ ghT,
-                                                      long long chunks, float* __restrict__ map,
-                                                      int* __restrict__ drop) {
-  __shared__ float sA[kWarps][32 * E], sC[kWarps][32 * E];
-  __shared__ int sDrop[kWarps];
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int c = (blockIdx.y * 32 + lane) * E;
+__global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate, Src<T> in, const float* __restrict__ s0,
+                                                      uint2* __restrict__ prefix, uint2* __restrict__ chunk) {
+  __shared__ uint2 sm[kThreads * E];
+  __shared__ uint2 seg[32 * E];  // segments x columns: 16 E, or 32 E where a warp takes a row
+  const int sub = threadIdx.x & (S.lanes - 1), per = kThreads / S.lanes, mine = threadIdx.x / S.lanes;
+  const int W = S.lanes * E, c = blockIdx.y * W + sub * E, warp_groups = S.lanes >= 32 ? 1 : 32 / S.lanes;
+  const long long g = blockIdx.x * (long long)per + mine, r0 = g * kGroup;
   const bool col = c < S.D;
-  const long long r0 = blockIdx.x * (long long)kRows + wid * kWarpRows;
-  const RowFlags f = row_flags(S, r0, lane);
-  float A[E], C[E];
+  const Edges ed = group_edges(S, g - mine % warp_groups, warp_groups, mine % warp_groups);
+  const unsigned edge = (BWD ? ed.last : ed.first) | ed.none;
+  float A[E], s[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) { A[e] = 1.f; C[e] = 0.f; }
-  bool cut = false;
+  for (int e = 0; e < E; ++e) { A[e] = 1.f; s[e] = 0.f; }
+  auto rows = [&](auto plain) {
+#pragma unroll 1
+    for (int q = 0; q < kGroup; q += kAhead) {
+      Pack<T, E> gp[kAhead], ip[kAhead];
 #pragma unroll
-  for (int k = 0; k < kWarpRows; ++k) {
-    const int i = BWD ? kWarpRows - 1 - k : k;
-    const long long n = r0 + i;
-    const bool valid = f.valid >> i & 1, edge = (BWD ? f.last : f.first) >> i & 1;
-    const int w = __shfl_sync(0xffffffffu, f.win, i);
-    if (n >= S.N) continue;
-    if (!valid) {
-      cut = true;
-#pragma unroll
-      for (int e = 0; e < E; ++e) C[e] = 0.f;
-      continue;
-    }
-    const Pack<T, E> gp = load_row<T, E>(gate, ldg, n, c, col), ip = load_row<T, E>(in, ldi, n, c, col);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float a, q;
-      row_coeff<KIND>(to_f32(gp.v[e]), &a, &q);
-      const float v = to_f32(ip.v[e]);
-      if (BWD) {  // u = a (dh + u_next)
-        const float nx = edge ? (ghT && col ? ghT[(long long)w * S.D + c + e] : 0.f) : C[e];
-        C[e] = a * (v + nx);
-      } else {
-        const float pv = edge ? (h0 && col ? h0[(long long)w * S.D + c + e] : 0.f) : C[e];
-        C[e] = fmaf(a, pv, KIND == ATLB_REC_SIGMOID ? q * v : v);
+      for (int j = 0; j < kAhead; ++j) {
+        const int r = BWD ? kGroup - 1 - q - j : q + j;
+        const bool ok = col && (decltype(plain)::value || !(ed.none >> r & 1));
+        gp[j] = load_or_zero<T, E>(gate.p + (r0 + r) * gate.ld + c, ok);
+        ip[j] = load_or_zero<T, E>(in.p + (r0 + r) * in.ld + c, ok);
       }
-      A[e] *= a;
-    }
-    cut = cut || edge;
-  }
 #pragma unroll
-  for (int e = 0; e < E; ++e) { sA[wid][lane * E + e] = A[e]; sC[wid][lane * E + e] = C[e]; }
-  if (lane == 0) sDrop[wid] = cut;
-  __syncthreads();
-  if (wid == 0 && col) {
-    bool d = false;
-    float a[E], s[E];
+      for (int j = 0; j < kAhead; ++j) {
+        const int r = BWD ? kGroup - 1 - q - j : q + j;
+        if (!decltype(plain)::value && (edge >> r & 1)) {
+          const bool ok = col && !(ed.none >> r & 1);
+          load_state(s0, ok ? window_of(S, r0 + r) : 0, S.D, c, ok, s);
+        }
 #pragma unroll
-    for (int e = 0; e < E; ++e) { a[e] = 1.f; s[e] = 0.f; }
-    for (int k = 0; k < kWarps; ++k) {
-      const int w = BWD ? kWarps - 1 - k : k;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        s[e] = sDrop[w] ? sC[w][lane * E + e] : through(sA[w][lane * E + e], sC[w][lane * E + e], s[e]);
-        a[e] *= sA[w][lane * E + e];
-      }
-      d = d || sDrop[w];
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      map[blockIdx.x * (long long)S.D + c + e] = a[e];
-      map[(chunks + blockIdx.x) * (long long)S.D + c + e] = s[e];
-    }
-    if (lane == 0 && blockIdx.y == 0) drop[blockIdx.x] = d;
-  }
-}
-
-// Chains the maps: state[chunk] is what enters the chunk (from the left, or BWD from the right).
-template <bool BWD>
-__global__ void __launch_bounds__(kThreads) k_rec_chain(const float* __restrict__ map, const int* __restrict__ drop,
-                                                        long long chunks, int D, float* __restrict__ state) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= D) return;
-  float s = 0.f;
-  for (long long k = 0; k < chunks; ++k) {
-    const long long q = BWD ? chunks - 1 - k : k;
-    state[q * D + c] = s;
-    const float A = map[q * D + c], C = map[(chunks + q) * D + c];
-    s = drop[q] ? C : through(A, C, s);
-  }
-}
-
-// The state that enters a warp's rows: the chunk's, passed through the warps before it (BWD: after it).
-template <int E, bool BWD>
-__device__ __forceinline__ void warp_state(const float (*sA)[32 * E], const float (*sC)[32 * E], const int* sDrop,
-                                           int wid, int lane, float (&s)[E]) {
-  for (int k = 0; k < (BWD ? kWarps - 1 - wid : wid); ++k) {
-    const int w = BWD ? kWarps - 1 - k : k;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      s[e] = sDrop[w] ? sC[w][lane * E + e] : through(sA[w][lane * E + e], sC[w][lane * E + e], s[e]);
-  }
-}
-
-template <typename T, int E, int KIND>
-__global__ void __launch_bounds__(kThreads) k_rec_fwd(RecShape S, const T* __restrict__ gate, long long ldg,
-                                                      const T* __restrict__ x, long long ldx,
-                                                      const float* __restrict__ h0, const float* __restrict__ state,
-                                                      T* __restrict__ h, float* __restrict__ hT) {
-  __shared__ float sA[kWarps][32 * E], sC[kWarps][32 * E];
-  __shared__ int sDrop[kWarps];
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int c = (blockIdx.y * 32 + lane) * E;
-  const bool col = c < S.D;
-  const long long r0 = blockIdx.x * (long long)kRows + wid * kWarpRows;
-  const RowFlags f = row_flags(S, r0, lane);
-  Pack<T, E> gp[kWarpRows], xp[kWarpRows];
-#pragma unroll
-  for (int i = 0; i < kWarpRows; ++i) {
-    const bool in = col && (f.valid >> i & 1);
-    gp[i] = load_row<T, E>(gate, ldg, r0 + i, c, in);
-    xp[i] = load_row<T, E>(x, ldx, r0 + i, c, in);
-  }
-  float s[E];
-#pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {  // the warp's map, then the rows from their true state
-    float A[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      A[e] = 1.f;
-      if (pass == 0) s[e] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kWarpRows; ++i) {
-      const int w = __shfl_sync(0xffffffffu, f.win, i);
-      const bool valid = f.valid >> i & 1, first = f.first >> i & 1, last = f.last >> i & 1;
-      Pack<T, E> out;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float a, q;
-        row_coeff<KIND>(to_f32(gp[i].v[e]), &a, &q);
-        const float v = to_f32(xp[i].v[e]);
-        const float pv = first ? (h0 && col && valid ? h0[(long long)w * S.D + c + e] : 0.f) : s[e];
-        s[e] = valid ? fmaf(a, pv, KIND == ATLB_REC_SIGMOID ? q * v : v) : 0.f;
-        A[e] *= a;
-        out.v[e] = from_f32<T>(s[e]);
-      }
-      if (pass == 1 && col && r0 + i < S.N) {
-        store_pack(h + (r0 + i) * S.D + c, out);
-        if (hT && last && valid) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) hT[(long long)w * S.D + c + e] = s[e];
+        for (int e = 0; e < E; ++e) {
+          float a, w, v;
+          row_terms<KIND>(to_f32(gp[j].v[e]), to_f32(ip[j].v[e]), &a, &w, &v);
+          s[e] = BWD ? a * (to_f32(ip[j].v[e]) + s[e]) : fmaf(a, s[e], v);
+          A[e] *= a;
         }
       }
     }
-    if (pass == 0) {
+  };
+  if (__any_sync(0xffffffffu, edge != 0))
+    rows(std::false_type());
+  else
+    rows(std::true_type());
+  // joined along the walk, per column: kSeg groups by one thread, then the segments, then the groups again
+  const int at = BWD ? per - 1 - mine : mine, segs = (per + kSeg - 1) / kSeg;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        sA[wid][lane * E + e] = A[e];
-        sC[wid][lane * E + e] = s[e];
-      }
-      if (lane == 0) sDrop[wid] = f.first != 0;
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < E; ++e) s[e] = col ? state[blockIdx.x * (long long)S.D + c + e] : 0.f;
-      warp_state<E, false>(sA, sC, sDrop, wid, lane, s);
+  for (int e = 0; e < E; ++e) sm[at * W + sub * E + e] = pack_map(Map{A[e], s[e], edge != 0});
+  __syncthreads();
+  for (int i = threadIdx.x; i < segs * W; i += kThreads) {
+    const int x = i % W, k0 = i / W * kSeg;
+    Map m = identity();
+    for (int k = k0; k < k0 + kSeg && k < per; ++k) {
+      const Map next = unpack_map(sm[k * W + x]);
+      sm[k * W + x] = pack_map(m);
+      m = then(m, next);
     }
-  }
-}
-
-template <typename T, int E, int KIND>
-__global__ void __launch_bounds__(kThreads) k_rec_bwd(RecShape S, const T* __restrict__ gate, long long ldg,
-                                                      const T* __restrict__ x, long long ldx,
-                                                      const T* __restrict__ gh, long long ldgh,
-                                                      const float* __restrict__ h0, const float* __restrict__ ghT,
-                                                      const float* __restrict__ saved,
-                                                      const float* __restrict__ state, T* __restrict__ ggate,
-                                                      T* __restrict__ gx, float* __restrict__ gh0) {
-  __shared__ float sA[kWarps][32 * E], sC[kWarps][32 * E], sU[kWarps][32 * E];
-  __shared__ int sDrop[kWarps], sDropU[kWarps];
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int c = (blockIdx.y * 32 + lane) * E;
-  const bool col = c < S.D;
-  const long long r0 = blockIdx.x * (long long)kRows + wid * kWarpRows;
-  const RowFlags f = row_flags(S, r0, lane);
-  Pack<T, E> gp[kWarpRows], xp[kWarpRows], dp[kWarpRows];
-#pragma unroll
-  for (int i = 0; i < kWarpRows; ++i) {
-    const bool in = col && (f.valid >> i & 1);
-    gp[i] = load_row<T, E>(gate, ldg, r0 + i, c, in);
-    xp[i] = load_row<T, E>(x, ldx, r0 + i, c, in);
-    dp[i] = load_row<T, E>(gh, ldgh, r0 + i, c, in);
-  }
-  float s[E], u[E], A[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) { s[e] = 0.f; u[e] = 0.f; A[e] = 1.f; }
-  // the warp's two maps
-#pragma unroll
-  for (int i = 0; i < kWarpRows; ++i) {
-    const int w = __shfl_sync(0xffffffffu, f.win, i);
-    const bool valid = f.valid >> i & 1, first = f.first >> i & 1;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float a, q;
-      row_coeff<KIND>(to_f32(gp[i].v[e]), &a, &q);
-      const float v = to_f32(xp[i].v[e]);
-      const float pv = first ? (h0 && col && valid ? h0[(long long)w * S.D + c + e] : 0.f) : s[e];
-      s[e] = valid ? fmaf(a, pv, KIND == ATLB_REC_SIGMOID ? q * v : v) : 0.f;
-      A[e] *= a;
-    }
-  }
-#pragma unroll
-  for (int i = kWarpRows - 1; i >= 0; --i) {
-    const int w = __shfl_sync(0xffffffffu, f.win, i);
-    const bool valid = f.valid >> i & 1, last = f.last >> i & 1;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float a, q;
-      row_coeff<KIND>(to_f32(gp[i].v[e]), &a, &q);
-      const float nx = last ? (ghT && col && valid ? ghT[(long long)w * S.D + c + e] : 0.f) : u[e];
-      u[e] = valid ? a * (to_f32(dp[i].v[e]) + nx) : 0.f;
-      if (r0 + i >= S.N) u[e] = 0.f;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    sA[wid][lane * E + e] = A[e];
-    sC[wid][lane * E + e] = s[e];
-    sU[wid][lane * E + e] = u[e];
-  }
-  if (lane == 0) {
-    sDrop[wid] = f.first != 0;
-    sDropU[wid] = f.last != 0 || r0 + kWarpRows > S.N;
+    seg[i] = pack_map(m);
   }
   __syncthreads();
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    s[e] = col ? saved[blockIdx.x * (long long)S.D + c + e] : 0.f;
-    u[e] = col ? state[blockIdx.x * (long long)S.D + c + e] : 0.f;
+  for (int x = threadIdx.x; x < W; x += kThreads) {
+    Map m = identity();
+    for (int k = 0; k < segs; ++k) {
+      const Map next = unpack_map(seg[k * W + x]);
+      seg[k * W + x] = pack_map(m);
+      m = then(m, next);
+    }
+    if (blockIdx.y * W + x < S.D) chunk[blockIdx.x * (long long)S.D + blockIdx.y * W + x] = pack_map(m);
   }
-  warp_state<E, false>(sA, sC, sDrop, wid, lane, s);
-  warp_state<E, true>(sA, sU, sDropU, wid, lane, u);
-  float hp[kWarpRows][E];  // h before each row
+  __syncthreads();
+  if (col && g < S.groups) {
 #pragma unroll
-  for (int i = 0; i < kWarpRows; ++i) {
-    const int w = __shfl_sync(0xffffffffu, f.win, i);
-    const bool valid = f.valid >> i & 1, first = f.first >> i & 1;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float a, q;
-      row_coeff<KIND>(to_f32(gp[i].v[e]), &a, &q);
-      const float v = to_f32(xp[i].v[e]);
-      hp[i][e] = first ? (h0 && col && valid ? h0[(long long)w * S.D + c + e] : 0.f) : s[e];
-      s[e] = valid ? fmaf(a, hp[i][e], KIND == ATLB_REC_SIGMOID ? q * v : v) : 0.f;
-    }
-  }
-#pragma unroll
-  for (int i = kWarpRows - 1; i >= 0; --i) {
-    const int w = __shfl_sync(0xffffffffu, f.win, i);
-    const bool valid = f.valid >> i & 1, first = f.first >> i & 1, last = f.last >> i & 1;
-    Pack<T, E> og, ox;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float a, q;
-      row_coeff<KIND>(to_f32(gp[i].v[e]), &a, &q);
-      const float nx = last ? (ghT && col && valid ? ghT[(long long)w * S.D + c + e] : 0.f) : u[e];
-      const float g = to_f32(dp[i].v[e]) + nx;
-      u[e] = valid && r0 + i < S.N ? a * g : 0.f;
-      float dg, dx;
-      if (KIND == ATLB_REC_SIGMOID) {
-        dg = g * (hp[i][e] - to_f32(xp[i].v[e])) * a * q;
-        dx = g * q;
-      } else {
-        dg = g * hp[i][e];
-        dx = g;
-      }
-      og.v[e] = from_f32<T>(valid ? dg : 0.f);
-      ox.v[e] = from_f32<T>(valid ? dx : 0.f);
-    }
-    if (col && r0 + i < S.N) {
-      store_pack(ggate + (r0 + i) * S.D + c, og);
-      store_pack(gx + (r0 + i) * S.D + c, ox);
-      if (gh0 && first && valid) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) gh0[(long long)w * S.D + c + e] = u[e];
-      }
-    }
+    for (int e = 0; e < E; ++e)
+      prefix[g * S.D + c + e] =
+          pack_map(then(unpack_map(seg[at / kSeg * W + sub * E + e]), unpack_map(sm[at * W + sub * E + e])));
   }
 }
 
-long long chunks_of(long long N) { return (N + kRows - 1) / kRows; }
+// ------------------------------------------------------------------------------------------------ between the chunks
+// state[k]: what enters chunk k along the walk.  Per column kChainSegs threads each join a run of chunks, the runs are
+// joined in order, and every thread walks its run again from the true state.
+template <bool BWD>
+__global__ void __launch_bounds__(kChainCols * kChainSegs) k_rec_chain(const uint2* __restrict__ chunk, int chunks, int D,
+                                                                       float* __restrict__ state) {
+  __shared__ uint2 sm[kChainSegs][kChainCols];
+  __shared__ float in[kChainSegs][kChainCols];
+  const int x = threadIdx.x % kChainCols, sg = threadIdx.x / kChainCols, c = blockIdx.x * kChainCols + x;
+  const int run = (chunks + kChainSegs - 1) / kChainSegs, k0 = sg * run, k1 = min(k0 + run, chunks);
+  auto at = [&](int k) { return (long long)(BWD ? chunks - 1 - k : k) * D + c; };
+  Map m = identity();
+  if (c < D) {
+#pragma unroll 8
+    for (int k = k0; k < k1; ++k) m = then(m, unpack_map(chunk[at(k)]));
+  }
+  sm[sg][x] = pack_map(m);
+  __syncthreads();
+  if (threadIdx.x < kChainCols) {
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < kChainSegs; ++k) {
+      in[k][threadIdx.x] = s;
+      s = apply(unpack_map(sm[k][threadIdx.x]), s);
+    }
+  }
+  __syncthreads();
+  if (c >= D) return;
+  float s = in[sg][x];
+#pragma unroll 8
+  for (int k = k0; k < k1; ++k) {
+    const uint2 v = chunk[at(k)];
+    state[at(k)] = s;
+    s = apply(unpack_map(v), s);
+  }
+}
+
+// The state that enters group g: the chunk's, through the map from there.  per: groups of a chunk.
+template <int E>
+__device__ __forceinline__ void group_state(const RecShape& S, const uint2* prefix, const float* state, long long g,
+                                            int per, int c, bool in, float (&s)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    s[e] = 0.f;
+    if (in && S.linked)
+      s[e] = apply(unpack_map(prefix[g * S.D + c + e]), S.chunks > 1 ? state[g / per * S.D + c + e] : 0.f);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ replay, forward
+template <typename T, int E, int KIND>
+__global__ void __launch_bounds__(kThreads, 4) k_rec_fwd(RecShape S, Src<T> gate, Src<T> x, const float* __restrict__ h0,
+                                                      const uint2* __restrict__ prefix,
+                                                      const float* __restrict__ state, T* __restrict__ h,
+                                                      float* __restrict__ hT, float* __restrict__ saved) {
+  const int sub = threadIdx.x & (S.lanes - 1), per = kThreads / S.lanes, mine = threadIdx.x / S.lanes;
+  const int c = (blockIdx.y * S.lanes + sub) * E, warp_groups = S.lanes >= 32 ? 1 : 32 / S.lanes;
+  // from the last chunk to the first: what the maps' kernel read last may still be in L2
+  const long long g = (gridDim.x - 1 - blockIdx.x) * (long long)per + mine, r0 = g * kGroup;
+  const bool col = c < S.D;
+  const Edges ed = group_edges(S, g - mine % warp_groups, warp_groups, mine % warp_groups);
+  const unsigned edge = ed.first | ed.none;
+  float s[E];
+  group_state(S, prefix, state, g, per, c, col && g < S.groups, s);
+  auto rows = [&](auto plain) {
+#pragma unroll 1
+    for (int q = 0; q < kGroup; q += kAhead) {
+      Pack<T, E> gp[kAhead], xp[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const bool ok = col && (decltype(plain)::value || !(ed.none >> (q + j) & 1));
+        gp[j] = load_or_zero<T, E>(gate.p + (r0 + q + j) * gate.ld + c, ok);
+        xp[j] = load_or_zero<T, E>(x.p + (r0 + q + j) * x.ld + c, ok);
+      }
+      if (saved && q % kPart == 0 && col && r0 + q < S.N) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) saved[(r0 + q) / kPart * S.D + c + e] = s[e];
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int r = q + j;
+        if (!decltype(plain)::value && (edge >> r & 1)) {
+          const bool ok = col && !(ed.none >> r & 1);
+          load_state(h0, ok ? window_of(S, r0 + r) : 0, S.D, c, ok, s);
+        }
+        Pack<T, E> o;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          float a, w, v;
+          row_terms<KIND>(to_f32(gp[j].v[e]), to_f32(xp[j].v[e]), &a, &w, &v);
+          s[e] = fmaf(a, s[e], v);
+          o.v[e] = from_f32<T>(s[e]);
+        }
+        if (col && (decltype(plain)::value || r0 + r < S.N)) store_pack(h + (r0 + r) * S.D + c, o);
+        if (!decltype(plain)::value && hT && col && (ed.last & ~ed.none) >> r & 1) {
+          const int win = window_of(S, r0 + r);
+#pragma unroll
+          for (int e = 0; e < E; ++e) hT[(long long)win * S.D + c + e] = s[e];
+        }
+      }
+    }
+  };
+  if (__any_sync(0xffffffffu, (edge | (hT ? ed.last : 0)) != 0))
+    rows(std::false_type());
+  else
+    rows(std::true_type());
+}
+
+// ------------------------------------------------------------------------------------------------ replay, backward
+// lanes_b threads on a row, E columns each (4 bytes), a group per `lanes_b` threads.  Each part of the group, the last
+// one first: its rows in registers, the states forward from the one the forward pass kept, then u backward.
+template <typename T, int E, int KIND>
+__global__ void __launch_bounds__(kThreads, 4) k_rec_bwd(RecShape S, int lanes_b, Src<T> gate, Src<T> x, Src<T> gh,
+                                                         const float* __restrict__ h0, const float* __restrict__ ghT,
+                                                         const float* __restrict__ saved,
+                                                         const uint2* __restrict__ prefix,
+                                                         const float* __restrict__ state, T* __restrict__ ggate,
+                                                         T* __restrict__ gx, float* __restrict__ gh0) {
+  const int sub = threadIdx.x & (lanes_b - 1), per = kThreads / lanes_b, mine = threadIdx.x / lanes_b;
+  const int c = (blockIdx.y * lanes_b + sub) * E, warp_groups = 32 / lanes_b;
+  // from the first chunk to the last: the maps' kernel walked towards the first
+  const long long g = blockIdx.x * (long long)per + mine, r0 = g * kGroup;
+  const bool col = c < S.D;
+  const Edges ed = group_edges(S, g - mine % warp_groups, warp_groups, mine % warp_groups);
+  const unsigned edge = ed.first | ed.none, edge_u = ed.last | ed.none;
+  float u[E];
+  group_state(S, prefix, state, g, kThreads / S.lanes, c, col && g < S.groups, u);
+  auto part = [&](int lo, auto plain) {
+    Pack<T, E> gp[kPart], xp[kPart], dp[kPart];
+    float hp[kPart][E], s[E];
+#pragma unroll
+    for (int r = 0; r < kPart; ++r) {
+      const bool ok = col && (decltype(plain)::value || !(ed.none >> (lo + r) & 1));
+      gp[r] = load_or_zero<T, E>(gate.p + (r0 + lo + r) * gate.ld + c, ok);
+      xp[r] = load_or_zero<T, E>(x.p + (r0 + lo + r) * x.ld + c, ok);
+      dp[r] = load_or_zero<T, E>(gh.p + (r0 + lo + r) * gh.ld + c, ok);
+    }
+    load_state(saved, (r0 + lo) / kPart, S.D, c, col && r0 + lo < S.N, s);
+#pragma unroll
+    for (int r = 0; r < kPart; ++r) {
+      if (!decltype(plain)::value && (edge >> (lo + r) & 1)) {
+        const bool ok = col && !(ed.none >> (lo + r) & 1);
+        load_state(h0, ok ? window_of(S, r0 + lo + r) : 0, S.D, c, ok, s);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float a, w, v;
+        row_terms<KIND>(to_f32(gp[r].v[e]), to_f32(xp[r].v[e]), &a, &w, &v);
+        hp[r][e] = s[e];
+        s[e] = fmaf(a, s[e], v);
+      }
+    }
+#pragma unroll
+    for (int r = kPart - 1; r >= 0; --r) {
+      if (!decltype(plain)::value && (edge_u >> (lo + r) & 1)) {
+        const bool ok = col && !(ed.none >> (lo + r) & 1);
+        load_state(ghT, ok ? window_of(S, r0 + lo + r) : 0, S.D, c, ok, u);
+      }
+      Pack<T, E> og, ox;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float a, w, v;
+        const float xv = to_f32(xp[r].v[e]), gt = to_f32(dp[r].v[e]) + u[e];
+        row_terms<KIND>(to_f32(gp[r].v[e]), xv, &a, &w, &v);
+        u[e] = a * gt;
+        og.v[e] = from_f32<T>(KIND == ATLB_REC_SIGMOID ? u[e] * (w * (hp[r][e] - xv)) : gt * hp[r][e]);
+        ox.v[e] = from_f32<T>(KIND == ATLB_REC_SIGMOID ? gt * w : gt);
+      }
+      if (col && (decltype(plain)::value || r0 + lo + r < S.N)) {
+        store_pack(ggate + (r0 + lo + r) * S.D + c, og);
+        store_pack(gx + (r0 + lo + r) * S.D + c, ox);
+      }
+      if (!decltype(plain)::value && gh0 && col && (ed.first & ~ed.none) >> (lo + r) & 1) {
+        const int win = window_of(S, r0 + lo + r);
+#pragma unroll
+        for (int e = 0; e < E; ++e) gh0[(long long)win * S.D + c + e] = u[e];
+      }
+    }
+  };
+  const bool some = __any_sync(0xffffffffu, (edge | edge_u) != 0);
+#pragma unroll 1
+  for (int lo = kGroup - kPart; lo >= 0; lo -= kPart) {
+    if (some)
+      part(lo, std::false_type());
+    else
+      part(lo, std::true_type());
+  }
+}
+
+long long groups_of(long long N) { return (N + kGroup - 1) / kGroup; }
 
 struct RecWs {
-  float *map, *state;
-  int* drop;
+  uint2 *prefix, *chunk;
+  float* state;
   size_t bytes;
 };
 
+// Room for chunks of the fewest groups (32 threads on a row).
 RecWs carve(void* ws, long long N, long long D) {
   Carve c(ws);
   RecWs w;
-  const long long k = chunks_of(N);
-  w.map = c.take<float>(2 * k * D);
+  const long long g = groups_of(N), k = (g + kThreads / 32 - 1) / (kThreads / 32);
+  w.prefix = c.take<uint2>(g * D);
+  w.chunk = c.take<uint2>(k * D);
   w.state = c.take<float>(k * D);
-  w.drop = c.take<int>(k);
   w.bytes = c.bytes_needed();
   return w;
 }
@@ -418,10 +450,54 @@ int with_kind(int kind, Fn&& fn) {
   return fn(std::integral_constant<int, ATLB_REC_DECAY>());
 }
 
+// The bytes that every row of the arrays and D are whole multiples of.
+struct Unit {
+  long long bits;
+  template <typename T>
+  void add(const void* p, long long ld) { bits |= (long long)(reinterpret_cast<uintptr_t>(p) | (ld * sizeof(T))); }
+  bool fits(int bytes) const { return bits % bytes == 0; }
+};
+
+// Lanes on a row of D columns with E each: a power of two, at most `most`.
+int lanes_for(long long D, int E, int most) {
+  int l = 1;
+  while (l < most && l * E < D) l *= 2;
+  return l;
+}
+
+// Shape for k_rec_map and k_rec_fwd with E columns per thread: 16 threads read a whole 128-byte line of a row, single
+// columns take a whole warp.  16 bytes per thread halve the warps that fit and measured 14 % slower.
+RecShape make_shape(long long N, long long B, long long D, const long long* b, int E) {
+  RecShape S;
+  S.N = N;
+  S.T = b ? 0 : (unsigned)(N / B);
+  S.B = (int)B;
+  S.D = (int)D;
+  S.b = b;
+  S.lanes = lanes_for(D, E, E > 1 ? 128 / kBytes : 32);
+  S.groups = (int)groups_of(N);
+  S.chunks = (S.groups + kThreads / S.lanes - 1) / (kThreads / S.lanes);
+  S.linked = S.groups > 1 && (b || kGroup % S.T != 0);
+  return S;
+}
+
+template <typename T, int E, int KIND, bool BWD>
+void find_states(const RecShape& S, Src<T> gate, Src<T> in, const float* s0, const RecWs& w, cudaStream_t s) {
+  if (!S.linked) return;
+  const int W = S.lanes * E;
+  launch(k_rec_map<T, E, KIND, BWD>, dim3(S.chunks, (S.D + W - 1) / W), kThreads, 0, s, S, gate, in, s0, w.prefix,
+         w.chunk);
+  if (S.chunks > 1)
+    launch(k_rec_chain<BWD>, (S.D + kChainCols - 1) / kChainCols, kChainCols * kChainSegs, 0, s, w.chunk, S.chunks, S.D,
+           w.state);
+}
+
 }  // namespace
 
 size_t recurrence_workspace_bytes(long long N, long long D) { return carve(nullptr, N, D).bytes; }
-size_t recurrence_saved_bytes(long long N, long long D) { return (size_t)chunks_of(N) * D * sizeof(float); }
+size_t recurrence_saved_bytes(long long N, long long D) {
+  return (size_t)((N + kPart - 1) / kPart) * D * sizeof(float);
+}
 
 int recurrence_fwd(int dtype, int kind, const void* gate, long long ldg, const void* x, long long ldx,
                    const long long* b, long long N, long long B, long long D, const float* h0, void* h, float* hT,
@@ -429,29 +505,26 @@ int recurrence_fwd(int dtype, int kind, const void* gate, long long ldg, const v
   if (D <= 0) return ATLB_OK;
   if (int st = fill_state(hT, h0, B * D, s)) return st;
   if (N <= 0) return ATLB_OK;
-  const RecShape S{N, b ? 0 : N / B, (int)B, (int)D, b};
   const RecWs w = carve(ws, N, D);
-  const long long k = chunks_of(N);
-  float* state = saved ? saved : w.state;
   return with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
+    Unit u{0};
+    u.add<T>(gate, ldg);
+    u.add<T>(x, ldx);
+    u.add<T>(h, D);
     return with_kind(kind, [&](auto kd) {
       constexpr int KIND = decltype(kd)::value;
+      const Src<T> sg{(const T*)gate, ldg}, sx{(const T*)x, ldx};
       auto go = [&](auto el) {
         constexpr int E = decltype(el)::value;
-        const dim3 grid((unsigned)k, (unsigned)((D + 32 * E - 1) / (32 * E)));
-        launch(k_rec_map<T, E, KIND, false>, grid, kThreads, 0, s, S, (const T*)gate, ldg, (const T*)x, ldx, h0,
-               (const float*)nullptr, k, w.map, w.drop);
-        launch(k_rec_chain<false>, (unsigned)((D + kThreads - 1) / kThreads), kThreads, 0, s, w.map, w.drop, k, (int)D,
-               state);
-        launch(k_rec_fwd<T, E, KIND>, grid, kThreads, 0, s, S, (const T*)gate, ldg, (const T*)x, ldx, h0, state,
-               (T*)h, hT);
+        const RecShape S = make_shape(N, B, D, b, E);
+        const int W = S.lanes * E;
+        find_states<T, E, KIND, false>(S, sg, sx, h0, w, s);
+        launch(k_rec_fwd<T, E, KIND>, dim3(S.chunks, (S.D + W - 1) / W), kThreads, 0, s, S, sg, sx, h0, w.prefix, w.state,
+               (T*)h, hT, saved);
         return launch_status("recurrence_fwd");
       };
-      if constexpr (sizeof(T) == 2) {
-        if (D % 2 == 0 && ldg % 2 == 0 && ldx % 2 == 0 && aligned_to(gate, 4) && aligned_to(x, 4) && aligned_to(h, 4))
-          return go(std::integral_constant<int, 2>());
-      }
+      if (u.fits(kBytes)) return go(std::integral_constant<int, kBytes / sizeof(T)>());
       return go(std::integral_constant<int, 1>());
     });
   });
@@ -464,28 +537,36 @@ int recurrence_bwd(int dtype, int kind, const void* gate, long long ldg, const v
   if (D <= 0) return ATLB_OK;
   if (int st = fill_state(gh0, ghT, B * D, s)) return st;
   if (N <= 0) return ATLB_OK;
-  const RecShape S{N, b ? 0 : N / B, (int)B, (int)D, b};
   const RecWs w = carve(ws, N, D);
-  const long long k = chunks_of(N);
   return with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
+    Unit u{0};
+    u.add<T>(gate, ldg);
+    u.add<T>(x, ldx);
+    u.add<T>(gh, ldgh);
+    u.add<T>(ggate, D);
+    u.add<T>(gx, D);
     return with_kind(kind, [&](auto kd) {
       constexpr int KIND = decltype(kd)::value;
+      const Src<T> sg{(const T*)gate, ldg}, sx{(const T*)x, ldx}, sd{(const T*)gh, ldgh};
+      RecShape S;
+      if (u.fits(kBytes)) {
+        constexpr int E = kBytes / sizeof(T);
+        S = make_shape(N, B, D, b, E);
+        find_states<T, E, KIND, true>(S, sg, sd, ghT, w, s);
+      } else {
+        S = make_shape(N, B, D, b, 1);
+        find_states<T, 1, KIND, true>(S, sg, sd, ghT, w, s);
+      }
       auto go = [&](auto el) {
         constexpr int E = decltype(el)::value;
-        const dim3 grid((unsigned)k, (unsigned)((D + 32 * E - 1) / (32 * E)));
-        launch(k_rec_map<T, E, KIND, true>, grid, kThreads, 0, s, S, (const T*)gate, ldg, (const T*)gh, ldgh,
-               (const float*)nullptr, ghT, k, w.map, w.drop);
-        launch(k_rec_chain<true>, (unsigned)((D + kThreads - 1) / kThreads), kThreads, 0, s, w.map, w.drop, k, (int)D,
-               w.state);
-        launch(k_rec_bwd<T, E, KIND>, grid, kThreads, 0, s, S, (const T*)gate, ldg, (const T*)x, ldx, (const T*)gh,
-               ldgh, h0, ghT, saved, w.state, (T*)ggate, (T*)gx, gh0);
+        const int lanes = lanes_for(D, E, 32), per = kThreads / lanes;
+        launch(k_rec_bwd<T, E, KIND>, dim3((S.groups + per - 1) / per, (unsigned)((D + lanes * E - 1) / (lanes * E))),
+               kThreads, 0, s, S, lanes, sg, sx, sd, h0, ghT, saved, w.prefix, w.state, (T*)ggate, (T*)gx, gh0);
         return launch_status("recurrence_bwd");
       };
       if constexpr (sizeof(T) == 2) {
-        if (D % 2 == 0 && ldg % 2 == 0 && ldx % 2 == 0 && ldgh % 2 == 0 && aligned_to(gate, 4) && aligned_to(x, 4) &&
-            aligned_to(gh, 4) && aligned_to(ggate, 4) && aligned_to(gx, 4))
-          return go(std::integral_constant<int, 2>());
+        if (u.fits(4)) return go(std::integral_constant<int, 2>());
       }
       return go(std::integral_constant<int, 1>());
     });

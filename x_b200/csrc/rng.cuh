@@ -26,19 +26,32 @@ __host__ __device__ __forceinline__ void mulhilo32(unsigned a, unsigned b, unsig
   *lo = (unsigned)p;
 }
 
-__host__ __device__ __forceinline__ Philox4 philox4x32_10(Philox4 c, unsigned k0, unsigned k1) {
+constexpr unsigned kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;  // key increments (golden ratio, sqrt(3) - 1)
+
+__host__ __device__ __forceinline__ Philox4 philox_round(const Philox4& c, unsigned k0, unsigned k1) {
   constexpr unsigned kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u;  // round multipliers
-  constexpr unsigned kW0 = 0x9E3779B9u, kW1 = 0xBB67AE85u;  // key increments (golden ratio, sqrt(3) - 1)
+  unsigned hi0, lo0, hi1, lo1;
+  mulhilo32(kM0, c.x, &hi0, &lo0);
+  mulhilo32(kM1, c.z, &hi1, &lo1);
+  return Philox4{hi1 ^ c.y ^ k0, lo1, hi0 ^ c.w ^ k1, lo0};
+}
+
+__host__ __device__ __forceinline__ Philox4 philox4x32_10(Philox4 c, unsigned k0, unsigned k1) {
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
-    unsigned hi0, lo0, hi1, lo1;
-    mulhilo32(kM0, c.x, &hi0, &lo0);
-    mulhilo32(kM1, c.z, &hi1, &lo1);
-    c = Philox4{hi1 ^ c.y ^ k0, lo1, hi0 ^ c.w ^ k1, lo0};
-    k0 += kW0;
-    k1 += kW1;
+    c = philox_round(c, k0, k1);
+    k0 += kPhiloxW0;
+    k1 += kPhiloxW1;
   }
   return c;
+}
+
+// The keys of the ten rounds, two words each.
+inline void philox_keys(unsigned k0, unsigned k1, unsigned (&key)[20]) {
+  for (int r = 0; r < 10; ++r) {
+    key[2 * r] = k0 + r * kPhiloxW0;
+    key[2 * r + 1] = k1 + r * kPhiloxW1;
+  }
 }
 
 struct RngKey {

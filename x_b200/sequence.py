@@ -49,11 +49,18 @@ def _on(dev):
     return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
+def _stream(dev):
+    """The current stream of the device as an integer (a Stream object costs several microseconds to make)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _rows(t):
     """(t, row stride) with neighbouring elements in each row of the 2-D tensor; a copy where they are not."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    n, d = t.shape
+    ld, one = t.stride()
+    if d > 1 and one != 1:
+        return t.contiguous(), d
+    return t, ld if n > 1 else d
 
 
 def _addr(t):
@@ -68,10 +75,11 @@ def _wants_grad(*tensors):
 def _embedding_fwd(weight, idx, scale):
     w, ldw = _rows(weight)
     V, D = w.shape
-    with _on(w.device):
-        out = torch.empty(*idx.shape, D, dtype=w.dtype, device=w.device)
-        L.check(L.lib().atlb_embedding_fwd(L.DTYPES[w.dtype], w.data_ptr(), ldw, V, D, idx.data_ptr(), idx.numel(),
-                                           scale, out.data_ptr(), L.stream()), "embedding")
+    dev = w.device
+    with _on(dev):
+        out = torch.empty(*idx.shape, D, dtype=w.dtype, device=dev)
+        L.check(L.load_library().atlb_embedding_fwd(L.DTYPES[w.dtype], w.data_ptr(), ldw, V, D, idx.data_ptr(), idx.numel(),
+                                           scale, out.data_ptr(), _stream(dev)), "embedding")
     return out
 
 
@@ -89,13 +97,13 @@ class _Embedding(torch.autograd.Function):
         (V, D), scale = ctx.meta
         g, ldg = _rows(g.reshape(idx.numel(), D))
         N = idx.numel()
-        lib = L.lib()
-        with _on(g.device):
-            grad = torch.empty(V, D, dtype=g.dtype, device=g.device)
+        dev, lib = g.device, L.load_library()
+        with _on(dev):
+            grad = torch.empty(V, D, dtype=g.dtype, device=dev)
             nb = lib.atlb_embedding_workspace_bytes(N, V, D)
-            ws = L.workspace(nb, g.device)
+            ws = L.workspace(nb, dev)
             L.check(lib.atlb_embedding_bwd(L.DTYPES[g.dtype], g.data_ptr(), ldg, idx.data_ptr(), N, V, D, scale,
-                                           grad.data_ptr(), ws.data_ptr(), nb, L.stream()), "embedding_bwd")
+                                           grad.data_ptr(), ws.data_ptr(), nb, _stream(dev)), "embedding_bwd")
         return grad, None, None
 
 
@@ -120,12 +128,12 @@ def embedding(weight: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> to
 # ------------------------------------------------------------------------------------------- dropout
 def _dropout_run(x, residual, p, seed, call):
     x = x.contiguous()
-    dev_call = call if torch.is_tensor(call) else None
-    with _on(x.device):
+    dev, dev_call = x.device, call if torch.is_tensor(call) else None
+    with _on(dev):
         out = torch.empty_like(x)
-        L.check(L.lib().atlb_dropout(L.DTYPES[x.dtype], x.data_ptr(), _addr(residual), x.numel(), p, seed,
+        L.check(L.load_library().atlb_dropout(L.DTYPES[x.dtype], x.data_ptr(), _addr(residual), x.numel(), p, seed,
                                      0 if dev_call is not None else call, _addr(dev_call), out.data_ptr(),
-                                     L.stream()), "dropout")
+                                     _stream(dev)), "dropout")
     return out
 
 
@@ -181,7 +189,7 @@ def _recurrence_fwd(gate, x, b, B, h0, kind, want_state, save):
     gate, ldgate = _rows(gate)
     x, ldx = _rows(x)
     N, D = x.shape
-    dev, lib = x.device, L.lib()
+    dev, lib = x.device, L.load_library()
     with _on(dev):
         h = torch.empty(N, D, dtype=x.dtype, device=dev)
         hT = torch.empty(B, D, dtype=torch.float32, device=dev) if want_state else None
@@ -190,7 +198,7 @@ def _recurrence_fwd(gate, x, b, B, h0, kind, want_state, save):
         ws = L.workspace(nb, dev)
         L.check(lib.atlb_recurrence_fwd(L.DTYPES[x.dtype], kind, gate.data_ptr(), ldgate, x.data_ptr(), ldx, _addr(b),
                                         N, B, D, _addr(h0), h.data_ptr(), _addr(hT), _addr(saved), ws.data_ptr(), nb,
-                                        L.stream()), "linear_recurrence")
+                                        _stream(dev)), "linear_recurrence")
     return h, hT, saved
 
 
@@ -213,7 +221,7 @@ class _Recurrence(torch.autograd.Function):
         gh, ldgh = _rows(torch.zeros_like(x) if gh is None else gh)
         ghT = None if ghT is None else ghT.contiguous()
         N, D = x.shape
-        dev, lib = x.device, L.lib()
+        dev, lib = x.device, L.load_library()
         with _on(dev):
             ggate, gx = (torch.empty(N, D, dtype=x.dtype, device=dev) for _ in range(2))
             gh0 = torch.empty(B, D, dtype=torch.float32, device=dev) if h0 is not None else None
@@ -222,7 +230,7 @@ class _Recurrence(torch.autograd.Function):
             L.check(lib.atlb_recurrence_bwd(L.DTYPES[x.dtype], kind, gate.data_ptr(), ldgate, x.data_ptr(), ldx,
                                             _addr(b), N, B, D, _addr(h0), saved.data_ptr(), gh.data_ptr(), ldgh,
                                             _addr(ghT), ggate.data_ptr(), gx.data_ptr(), _addr(gh0), ws.data_ptr(), nb,
-                                            L.stream()), "linear_recurrence_bwd")
+                                            _stream(dev)), "linear_recurrence_bwd")
         return ggate, gx, None, None, gh0, None, None
 
 

@@ -661,9 +661,9 @@ size_t atlb_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D) {
   return embedding_workspace_bytes(N < 0 ? 0 : N, V < 0 ? 0 : V, D < 0 ? 0 : D);
 }
 
-static int check_rows(int64_t V, const char* fn) {
-  if (V >= (1LL << 31) - 1) {
-    set_error("%s: %lld table rows exceed the 32-bit row numbers", fn, (long long)V);
+static int check_rows(int64_t V, int64_t ld, const char* fn) {
+  if (V >= (1LL << 31) - 1 || ld > (1LL << 31) - 1) {
+    set_error("%s: %lld table rows or a row stride of %lld exceed 32 bits", fn, (long long)V, (long long)ld);
     return ATLB_ERR_OVERFLOW;
   }
   return ATLB_OK;
@@ -674,7 +674,7 @@ int atlb_embedding_fwd(int dtype, const void* weight, int64_t ldw, int64_t V, in
   clear();
   NONNEG(N); NONNEG(V); NONNEG(D); NONNEG(ldw);
   if (int st = check_seq(dtype, N, D, __func__)) return st;
-  if (int st = check_rows(V, __func__)) return st;
+  if (int st = check_rows(V, ldw, __func__)) return st;
   NEED(weight, V * D); NEED(idx, N); NEED(out, N * D);
   return embedding_fwd(dtype, weight, ldw, V, D, LL(idx), N, scale, out, STREAM(stream));
 }
@@ -684,7 +684,7 @@ int atlb_embedding_bwd(int dtype, const void* g, int64_t ldg, const int64_t* idx
   clear();
   NONNEG(N); NONNEG(V); NONNEG(D); NONNEG(ldg);
   if (int st = check_seq(dtype, N, D, __func__)) return st;
-  if (int st = check_rows(V, __func__)) return st;
+  if (int st = check_rows(V, ldg, __func__)) return st;
   NEED(g, N * D); NEED(idx, N); NEED(grad, V * D);
   if (int st = check_ws(workspace, workspace_bytes, embedding_workspace_bytes(N, V, D), __func__)) return st;
   return embedding_bwd(dtype, g, ldg, LL(idx), N, V, D, scale, grad, workspace, STREAM(stream));

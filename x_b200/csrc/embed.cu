@@ -14,33 +14,58 @@ namespace {
 constexpr int kThreads = 256;
 
 // ------------------------------------------------------------------------------------------------ forward
-// A group of `lanes` threads (a power of two up to 32) per row, E neighbouring elements per thread.
+// A group of `lanes` threads (a power of two up to 32) walks kRowsEach rows, E neighbouring columns per thread: the
+// rows' numbers, then all their loads, then the stores.
+constexpr int kRowsEach = 4;
+
 template <typename T, int E>
-__global__ void __launch_bounds__(kThreads) k_embed_fwd(const T* __restrict__ W, long long ldw, long long V, int D,
-                                                        const long long* __restrict__ idx, long long N, float scale,
-                                                        int lanes, T* __restrict__ out) {
+__global__ void __launch_bounds__(kThreads, 5) k_embed_fwd(const T* __restrict__ W, int ldw, int V, int D,
+                                                           const long long* __restrict__ idx, int N, float scale,
+                                                           int lanes, T* __restrict__ out) {
   const int sub = threadIdx.x & (lanes - 1), per = kThreads / lanes;
-  const long long stride = (long long)gridDim.x * per;
-  for (long long n = blockIdx.x * (long long)per + threadIdx.x / lanes; n < N; n += stride) {
-    const long long v = idx[n];
-    const bool ok = v >= 0 && v < V;
-    for (int c = sub * E; c < D; c += lanes * E) {
-      Pack<T, E> r;
-      if (ok) r = load_pack<T, E>(W + v * ldw + c);
+  const unsigned n0 = blockIdx.x * (unsigned)(per * kRowsEach) + threadIdx.x / lanes;
+  int v[kRowsEach];  // -1: no row
 #pragma unroll
-      for (int e = 0; e < E; ++e) r.v[e] = from_f32<T>(ok ? to_f32(r.v[e]) * scale : 0.f);
-      store_pack(out + n * D + c, r);
+  for (int k = 0; k < kRowsEach; ++k) {
+    const long long i = n0 + k * per < N ? __ldg(idx + n0 + k * per) : -1;
+    v[k] = i >= 0 && i < V ? (int)i : -1;
+  }
+  for (int c = (blockIdx.y * lanes + sub) * E; c < D; c += gridDim.y * lanes * E) {
+    Pack<T, E> r[kRowsEach];
+#pragma unroll
+    for (int k = 0; k < kRowsEach; ++k) {
+      if (v[k] >= 0) {
+        r[k] = load_pack<T, E>(W + (long long)v[k] * ldw + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) r[k].v[e] = from_f32<T>(0.f);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRowsEach; ++k) {
+      // a row outside the table stays zero whatever the scale
+      if (v[k] >= 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) r[k].v[e] = from_f32<T>(to_f32(r[k].v[e]) * scale);
+      }
+      if (n0 + k * per < N) store_pack(out + (long long)(n0 + k * per) * D + c, r[k]);
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ sort
-// Least-significant-digit radix sort of (row, event) pairs, up to kMaxBits per pass.  A tile is kTileItems
-// neighbouring pairs; every pass counts the tile's digits, scans the counts (digit-major) and places the pairs.
-constexpr int kItems = 8;
-constexpr int kTileItems = kThreads * kItems;
+// Least-significant-digit radix sort of (row, event) pairs, up to kMaxBits per pass.  A tile is 512 * ITEMS
+// neighbouring pairs; every pass counts the tile's digits, scans the counts (digit-major) and places the pairs.  Tiles
+// of 4096 pairs spread the work per digit (a place per warp and digit to clear and to sum) over more pairs; below 64 tiles
+// of that size the GPU would idle, and tiles of 2048 are taken.
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxBits = 10;
 constexpr int kMaxBins = 1 << kMaxBits;
+
+struct Pair {
+  unsigned row, event;
+};
 
 // Row numbers outside the table sort behind the last row.
 __device__ __forceinline__ unsigned row_key(long long v, unsigned V) {
@@ -48,27 +73,33 @@ __device__ __forceinline__ unsigned row_key(long long v, unsigned V) {
 }
 
 template <bool FIRST>
-__device__ __forceinline__ unsigned sort_key(const void* src, long long i, unsigned V) {
-  return FIRST ? row_key(static_cast<const long long*>(src)[i], V) : static_cast<const unsigned*>(src)[i];
+__device__ __forceinline__ Pair sort_pair(const void* src, long long i, unsigned V) {
+  if (FIRST) return Pair{row_key(__ldg(static_cast<const long long*>(src) + i), V), (unsigned)i};
+  const uint2 q = __ldg(static_cast<const uint2*>(src) + i);
+  return Pair{q.x, q.y};
 }
 
-template <bool FIRST>
-__global__ void __launch_bounds__(kThreads) k_sort_count(const void* __restrict__ src, long long N, unsigned V,
-                                                         int shift, int bins, int tiles, unsigned* __restrict__ counts) {
+template <bool FIRST, int ITEMS>
+__global__ void __launch_bounds__(kSortThreads) k_sort_count(const void* __restrict__ src, long long N, unsigned V,
+                                                             int shift, int bins, int tiles,
+                                                             unsigned* __restrict__ counts,
+                                                             unsigned* __restrict__ list_n) {
   __shared__ unsigned hist[kMaxBins];
-  for (int d = threadIdx.x; d < bins; d += kThreads) hist[d] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *list_n = 0;  // for the kernels behind the sort
+  for (int d = threadIdx.x; d < bins; d += kSortThreads) hist[d] = 0;
   __syncthreads();
-  const long long base = blockIdx.x * (long long)kTileItems;
+  const long long base = blockIdx.x * (long long)(kSortThreads * ITEMS);
 #pragma unroll
-  for (int r = 0; r < kItems; ++r) {
-    const long long i = base + r * kThreads + threadIdx.x;
-    if (i < N) atomicAdd(&hist[(sort_key<FIRST>(src, i, V) >> shift) & (bins - 1)], 1u);
+  for (int r = 0; r < ITEMS; ++r) {
+    const long long i = base + r * kSortThreads + threadIdx.x;
+    if (i < N) atomicAdd(&hist[(sort_pair<FIRST>(src, i, V).row >> shift) & (bins - 1)], 1u);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += kThreads) counts[(long long)d * tiles + blockIdx.x] = hist[d];
+  for (int d = threadIdx.x; d < bins; d += kSortThreads) counts[(long long)d * tiles + blockIdx.x] = hist[d];
 }
 
-// Exclusive sum over 256 threads; returns this thread's, *total the whole.
+// Exclusive sum over the CTA's THREADS threads; returns this thread's, *total the whole.
+template <int THREADS>
 __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* sm, unsigned* total) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   unsigned inc = v;
@@ -81,7 +112,7 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* sm, unsigne
   __syncthreads();
   unsigned before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < THREADS / 32; ++w) {
     if (w < wid) before += sm[w];
     all += sm[w];
   }
@@ -100,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) k_sort_scan(unsigned* __restrict__ c
     const int t = t0 + threadIdx.x;
     const unsigned v = t < tiles ? row[t] : 0;
     unsigned total;
-    const unsigned ex = block_scan(v, sm, &total);
+    const unsigned ex = block_scan<kThreads>(v, sm, &total);
     if (t < tiles) row[t] = carry + ex;
     carry += total;
   }
@@ -109,38 +140,36 @@ __global__ void __launch_bounds__(kThreads) k_sort_scan(unsigned* __restrict__ c
 
 // Stable placement: a warp ranks 32 neighbouring pairs at a time among equal digits (match), on top of the counts
 // of the rounds and warps before it.
-template <bool FIRST>
-__global__ void __launch_bounds__(kThreads) k_sort_place(const void* __restrict__ src, const unsigned* __restrict__ pos,
-                                                         long long N, unsigned V, int shift, int bins, int tiles,
-                                                         const unsigned* __restrict__ counts,
-                                                         const unsigned* __restrict__ totals,
-                                                         unsigned* __restrict__ key_out, unsigned* __restrict__ pos_out) {
-  constexpr int W = kThreads / 32;
-  __shared__ unsigned short hist[W][kMaxBins];
+template <bool FIRST, int ITEMS>
+__global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restrict__ src, long long N, unsigned V,
+                                                             int shift, int bins, int tiles,
+                                                             const unsigned* __restrict__ counts,
+                                                             const unsigned* __restrict__ totals,
+                                                             uint2* __restrict__ out) {
+  __shared__ unsigned short hist[kSortWarps][kMaxBins];
   __shared__ unsigned start[kMaxBins];
-  __shared__ unsigned sm[W];
+  __shared__ unsigned sm[kSortWarps];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  for (int d = threadIdx.x; d < bins; d += kThreads)
+  const long long base = blockIdx.x * (long long)(kSortThreads * ITEMS) + wid * (32 * ITEMS) + lane;
+  Pair p[ITEMS];
 #pragma unroll
-    for (int w = 0; w < W; ++w) hist[w][d] = 0;
+  for (int r = 0; r < ITEMS; ++r)
+    if (base + r * 32 < N) p[r] = sort_pair<FIRST>(src, base + r * 32, V);
+  for (int d = lane; d < bins; d += 32) hist[wid][d] = 0;
   unsigned carry = 0;
-  for (int d0 = 0; d0 < bins; d0 += kThreads) {
+  for (int d0 = 0; d0 < bins; d0 += kSortThreads) {
     const int d = d0 + threadIdx.x;
     unsigned total;
-    const unsigned ex = block_scan(d < bins ? totals[d] : 0, sm, &total);
+    const unsigned ex = block_scan<kSortThreads>(d < bins ? totals[d] : 0, sm, &total);
     if (d < bins) start[d] = carry + ex + counts[(long long)d * tiles + blockIdx.x];
     carry += total;
   }
-  __syncthreads();
-  const long long base = blockIdx.x * (long long)kTileItems + wid * (32 * kItems) + lane;
-  unsigned key[kItems], rank[kItems];
+  unsigned rank[ITEMS];
 #pragma unroll
-  for (int r = 0; r < kItems; ++r) {
-    const long long i = base + r * 32;
-    const bool in = i < N;
-    key[r] = in ? sort_key<FIRST>(src, i, V) : 0xffffffffu;
-    const unsigned d = (key[r] >> shift) & (bins - 1);
-    const unsigned peers = __match_any_sync(0xffffffffu, in ? d : 0xffffffffu);
+  for (int r = 0; r < ITEMS; ++r) {
+    const bool in = base + r * 32 < N;
+    const unsigned d = in ? (p[r].row >> shift) & (bins - 1) : 0xffffffffu;
+    const unsigned peers = __match_any_sync(0xffffffffu, d);
     unsigned before = 0;
     if (in) before = hist[wid][d];
     __syncwarp();
@@ -149,10 +178,10 @@ __global__ void __launch_bounds__(kThreads) k_sort_place(const void* __restrict_
     __syncwarp();
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += kThreads) {
+  for (int d = threadIdx.x; d < bins; d += kSortThreads) {
     unsigned c = 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
+    for (int w = 0; w < kSortWarps; ++w) {
       const unsigned h = hist[w][d];
       hist[w][d] = (unsigned short)c;
       c += h;
@@ -160,19 +189,17 @@ __global__ void __launch_bounds__(kThreads) k_sort_place(const void* __restrict_
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kItems; ++r) {
-    const long long i = base + r * 32;
-    if (i < N) {
-      const unsigned d = (key[r] >> shift) & (bins - 1);
-      const unsigned at = start[d] + hist[wid][d] + rank[r];
-      key_out[at] = key[r];
-      pos_out[at] = FIRST ? (unsigned)i : pos[i];
+  for (int r = 0; r < ITEMS; ++r) {
+    if (base + r * 32 < N) {
+      const unsigned d = (p[r].row >> shift) & (bins - 1);
+      out[start[d] + hist[wid][d] + rank[r]] = make_uint2(p[r].row, p[r].event);
     }
   }
 }
 
 struct SortPlan {
   int passes, bits, tiles;
+  bool large;  // tiles of 4096 pairs, else 2048
 };
 
 SortPlan sort_plan(long long N, long long V) {
@@ -181,7 +208,9 @@ SortPlan sort_plan(long long N, long long V) {
   SortPlan s;
   s.passes = (need + kMaxBits - 1) / kMaxBits;
   s.bits = (need + s.passes - 1) / s.passes;
-  s.tiles = (int)((N + kTileItems - 1) / kTileItems);
+  s.large = N > 64 * 4096;
+  const int tile = s.large ? 4096 : 2048;
+  s.tiles = (int)((N + tile - 1) / tile);
   return s;
 }
 
@@ -192,87 +221,147 @@ SortPlan sort_plan(long long N, long long V) {
 constexpr int kAhead = 4;  // rows in flight per thread
 
 template <typename T, int E>
-__global__ void __launch_bounds__(kThreads) k_embed_sum(const T* __restrict__ g, long long ldg,
-                                                        const unsigned* __restrict__ key,
-                                                        const unsigned* __restrict__ pos, long long N, unsigned V,
-                                                        int D, int L, int lanes, float scale, T* __restrict__ grad,
-                                                        float* __restrict__ part) {
+__global__ void __launch_bounds__(kThreads, 4) k_embed_sum(const T* __restrict__ g, int ldg,
+                                                           const uint2* __restrict__ pair, int N, unsigned V, int D,
+                                                           int L, int lanes, float scale, T* __restrict__ grad,
+                                                           float* __restrict__ part) {
   const int sub = threadIdx.x & (lanes - 1), per = kThreads / lanes;
-  const long long chunk = blockIdx.x * (long long)per + threadIdx.x / lanes;
+  const unsigned chunk = blockIdx.x * (unsigned)per + threadIdx.x / lanes;
   const int c = (blockIdx.y * lanes + sub) * E;
-  const long long j0 = chunk * L, j1 = j0 + L < N ? j0 + L : N;
-  if (j0 >= N || c >= D) return;
-  const unsigned prev = j0 > 0 ? key[j0 - 1] : 0xffffffffu, next = j1 < N ? key[j1] : 0xffffffffu;
-  unsigned cur = key[j0];
+  if ((long long)chunk * L >= N || c >= D) return;
+  const int j0 = chunk * L, j1 = min(N - j0, L) + j0;
+  const unsigned prev = j0 > 0 ? pair[j0 - 1].x : 0xffffffffu;
+  unsigned cur = pair[j0].x;
   bool head = cur == prev;
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  auto to_part = [&](int slot) {
-    float* p = part + (chunk * 2 + slot) * D + c;
+  auto put = [&](bool to_part, int slot) {
+    if (to_part) {
+      float* p = part + ((long long)chunk * 2 + slot) * D + c;
 #pragma unroll
-    for (int e = 0; e < E; ++e) p[e] = acc[e];
-  };
-  auto to_grad = [&]() {
-    Pack<T, E> r;
+      for (int e = 0; e < E; ++e) p[e] = acc[e];
+    } else {
+      Pack<T, E> r;
 #pragma unroll
-    for (int e = 0; e < E; ++e) r.v[e] = from_f32<T>(acc[e] * scale);
-    store_pack(grad + (long long)cur * D + c, r);
+      for (int e = 0; e < E; ++e) r.v[e] = from_f32<T>(acc[e] * scale);
+      store_pack(grad + (long long)cur * D + c, r);
+    }
   };
-  for (long long j = j0; j < j1 && cur < V; j += kAhead) {
-    unsigned k[kAhead];
+#pragma unroll 1
+  for (int j = j0; j < j1 && cur < V; j += kAhead) {
+    unsigned row[kAhead];
     Pack<T, E> r[kAhead];
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
-      k[q] = j + q < j1 ? key[j + q] : V;
-      if (k[q] < V) r[q] = load_pack<T, E>(g + (long long)pos[j + q] * ldg + c);
+      uint2 k = make_uint2(V, 0);
+      if (j + q < j1) k = __ldg(pair + j + q);
+      row[q] = k.x;
+      if (k.x < V) {
+        r[q] = load_pack<T, E>(g + (long long)k.y * ldg + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) r[q].v[e] = from_f32<T>(0.f);
+      }
     }
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
-      if (j + q >= j1) break;
-      if (k[q] != cur) {
-        if (cur < V) {
-          if (head) to_part(0);
-          else to_grad();
-        }
-        cur = k[q];
+      if (j + q < j1 && row[q] != cur) {
+        if (cur < V) put(head, 0);
+        cur = row[q];
         head = false;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = 0.f;
       }
-      if (k[q] < V) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += to_f32(r[q].v[e]);
-      }
+      for (int e = 0; e < E; ++e) acc[e] += to_f32(r[q].v[e]);
     }
   }
   if (cur >= V) return;
-  if (head) to_part(0);
-  else if (cur == next) to_part(1);
-  else to_grad();
+  const bool on = j1 < N && pair[j1].x == cur;  // goes on in the next chunk
+  put(head || on, head ? 0 : 1);
 }
 
-// The chunk in which a run over several chunks begins joins its partial sums, in order.
+// The chunk in which a run over several chunks begins joins its partial sums, in order: a warp per chunk.  Runs that go
+// on over kJoin chunks or more are put on a list for k_embed_join_long (in any order: each gives its own row).
+constexpr int kJoin = 32;
+struct LongRun {
+  unsigned chunk, row;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_embed_join(const unsigned* __restrict__ key, long long N, unsigned V,
-                                                         int D, int L, float scale, const float* __restrict__ part,
-                                                         T* __restrict__ grad) {
-  const long long chunk = blockIdx.x;
-  const long long j0 = chunk * L, j1 = j0 + L;
-  if (j1 >= N) return;
-  const unsigned cur = key[j1 - 1];
-  if (cur >= V || key[j1] != cur) return;
-  if (j0 > 0 && key[j0] == cur && key[j0 - 1] == cur) return;  // it began further left
-  for (int c = threadIdx.x; c < D; c += kThreads) {
-    float acc = part[(chunk * 2 + 1) * D + c];
-    for (long long e = chunk + 1; e * L < N && key[e * L] == cur; ++e) acc += part[e * 2 * D + c];
+__global__ void __launch_bounds__(kThreads) k_embed_join(const uint2* __restrict__ pair, int N, unsigned V, int D, int L,
+                                                         unsigned chunks, float scale, const float* __restrict__ part,
+                                                         T* __restrict__ grad, unsigned* __restrict__ list_n,
+                                                         LongRun* __restrict__ list) {
+  const unsigned chunk = blockIdx.x * (unsigned)(kThreads / 32) + threadIdx.x / 32;
+  const int lane = threadIdx.x & 31;
+  if (chunk + 1 >= chunks) return;
+  const int j0 = chunk * L, j1 = j0 + L;
+  const unsigned cur = pair[j1 - 1].x;
+  if (cur >= V || pair[j1].x != cur) return;
+  if (j0 > 0 && pair[j0].x == cur && pair[j0 - 1].x == cur) return;  // it began further left
+  // lane i: does the run go on into chunk + 2 + i?
+  const unsigned next = chunk + 2 + lane;
+  const unsigned stops = __ballot_sync(0xffffffffu, next >= chunks || pair[(long long)next * L].x != cur);
+  if (stops == 0) {
+    if (lane == 0) list[atomicAdd(list_n, 1u)] = LongRun{chunk, cur};
+    return;
+  }
+  const unsigned last = chunk + __ffs(stops);
+  for (int c = lane; c < D; c += 32) {
+    float acc = part[((long long)chunk * 2 + 1) * D + c];
+#pragma unroll 4
+    for (unsigned e = chunk + 1; e <= last; ++e) acc += part[(long long)e * 2 * D + c];
     grad[(long long)cur * D + c] = from_f32<T>(acc * scale);
   }
 }
 
+// Long runs, a CTA for each and 32 columns: 32 warps take every 32nd partial sum each, then their sums are added in
+// order.
+constexpr int kLongThreads = 1024;
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) k_embed_join_long(const uint2* __restrict__ pair, int D, int L,
+                                                                  unsigned chunks, float scale,
+                                                                  const float* __restrict__ part, T* __restrict__ grad,
+                                                                  const unsigned* __restrict__ list_n,
+                                                                  const LongRun* __restrict__ list) {
+  __shared__ float sm[32][33];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const unsigned n = *list_n;
+  for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
+    const LongRun run = list[i];
+    // the chunks it goes on into
+    unsigned last = run.chunk;
+    for (;;) {
+      const unsigned e = last + 1 + threadIdx.x;
+      const int more = __syncthreads_count(e < chunks && pair[(long long)e * L].x == run.row);
+      last += more;
+      if (more < kLongThreads) break;
+    }
+    for (int c0 = blockIdx.y * 32; c0 < D; c0 += gridDim.y * 32) {
+      const int c = c0 + lane;
+      float acc = 0.f;
+      if (c < D) {
+        if (wid == 0) acc = part[((long long)run.chunk * 2 + 1) * D + c];
+#pragma unroll 8
+        for (unsigned e = run.chunk + 1 + wid; e <= last; e += 32) acc += part[(long long)e * 2 * D + c];
+      }
+      sm[wid][lane] = acc;
+      __syncthreads();
+      if (wid == 0 && c < D) {
+        for (int w = 1; w < 32; ++w) acc += sm[w][lane];
+        grad[(long long)run.row * D + c] = from_f32<T>(acc * scale);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Pairs per chunk: about 16384 chunks where there are enough pairs, one wave of groups on the GPU.
 int sum_chunk(long long N) {
-  int L = 32;
-  while (L < (1 << 20) && N / L > 8192) L *= 2;
+  int L = 16;
+  while (L < (1 << 20) && N / L > 16384) L *= 2;
   return L;
 }
 
@@ -283,8 +372,10 @@ int group_lanes(int D, int E) {
 }
 
 struct EmbedWs {
-  unsigned *key[2], *pos[2], *counts, *totals;
+  uint2* pair[2];
+  unsigned *counts, *totals;
   float* part;
+  LongRun* list;
   size_t bytes;
 };
 
@@ -293,13 +384,11 @@ EmbedWs carve(void* ws, long long N, long long V, long long D) {
   const int L = sum_chunk(N);
   Carve c(ws);
   EmbedWs w;
-  for (int i = 0; i < 2; ++i) {
-    w.key[i] = c.take<unsigned>(N);
-    w.pos[i] = c.take<unsigned>(N);
-  }
+  for (int i = 0; i < 2; ++i) w.pair[i] = c.take<uint2>(s.passes > i ? N : 0);
   w.counts = c.take<unsigned>(((long long)s.tiles) << s.bits);
-  w.totals = c.take<unsigned>(1LL << s.bits);
+  w.totals = c.take<unsigned>((1LL << s.bits) + 1);  // and the length of the list of long runs
   w.part = c.take<float>((N + L - 1) / L * 2 * D);
+  w.list = c.take<LongRun>((N + L - 1) / L / kJoin + 1);
   w.bytes = c.bytes_needed();
   return w;
 }
@@ -316,11 +405,18 @@ int embedding_fwd(int dtype, const void* W, long long ldw, long long V, long lon
     constexpr int E = 16 / sizeof(T);
     const bool wide = D % E == 0 && ldw % E == 0 && aligned_to(W, 16) && aligned_to(out, 16);
     const int lanes = group_lanes((int)D, wide ? E : 1);
-    const int grid = clamp_grid((N + kThreads / lanes - 1) / (kThreads / lanes));
+    const long long per = kThreads / lanes * kRowsEach;
+    // few rows of many columns: the columns spread over CTAs as well
+    const int E1 = wide ? E : 1, slabs = (int)((D + lanes * E1 - 1) / (lanes * E1));
+    const dim3 grid((unsigned)((N + per - 1) / per), N < per * 148 ? (slabs < 65535 ? slabs : 65535) : 1);
+    auto go = [&](auto el) {
+      launch(k_embed_fwd<T, decltype(el)::value>, grid, kThreads, 0, s, (const T*)W, (int)ldw, (int)V, (int)D, idx, (int)N,
+             (float)scale, lanes, (T*)out);
+    };
     if (wide)
-      launch(k_embed_fwd<T, E>, grid, kThreads, 0, s, (const T*)W, ldw, V, (int)D, idx, N, (float)scale, lanes, (T*)out);
+      go(std::integral_constant<int, E>());
     else
-      launch(k_embed_fwd<T, 1>, grid, kThreads, 0, s, (const T*)W, ldw, V, (int)D, idx, N, (float)scale, lanes, (T*)out);
+      go(std::integral_constant<int, 1>());
     return launch_status("embedding_fwd");
   });
 }
@@ -334,22 +430,32 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
   const SortPlan p = sort_plan(N, V);
   const EmbedWs w = carve(ws, N, V, D);
   const int bins = 1 << p.bits, L = sum_chunk(N);
-  int at = 0;
+  unsigned* list_n = w.totals + bins;
+  const void* src = idx;
   for (int i = 0; i < p.passes; ++i) {
-    const int shift = i * p.bits;
-    if (i == 0) {
-      launch(k_sort_count<true>, p.tiles, kThreads, 0, s, (const void*)idx, N, (unsigned)V, shift, bins, p.tiles, w.counts);
+    uint2* dst = w.pair[i & 1];
+    auto pass = [&](auto first, auto items) {
+      constexpr bool F = decltype(first)::value;
+      constexpr int I = decltype(items)::value;
+      launch(k_sort_count<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, p.tiles, w.counts,
+             list_n);
       launch(k_sort_scan, bins, kThreads, 0, s, w.counts, p.tiles, w.totals);
-      launch(k_sort_place<true>, p.tiles, kThreads, 0, s, (const void*)idx, (const unsigned*)nullptr, N, (unsigned)V, shift,
-             bins, p.tiles, w.counts, w.totals, w.key[0], w.pos[0]);
-    } else {
-      launch(k_sort_count<false>, p.tiles, kThreads, 0, s, (const void*)w.key[at], N, (unsigned)V, shift, bins, p.tiles, w.counts);
-      launch(k_sort_scan, bins, kThreads, 0, s, w.counts, p.tiles, w.totals);
-      launch(k_sort_place<false>, p.tiles, kThreads, 0, s, (const void*)w.key[at], (const unsigned*)w.pos[at], N,
-             (unsigned)V, shift, bins, p.tiles, w.counts, w.totals, w.key[at ^ 1], w.pos[at ^ 1]);
-      at ^= 1;
-    }
+      launch(k_sort_place<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, p.tiles, w.counts,
+             w.totals, dst);
+    };
+    auto sized = [&](auto first) {
+      if (p.large)
+        pass(first, std::integral_constant<int, 8>());
+      else
+        pass(first, std::integral_constant<int, 4>());
+    };
+    if (i == 0)
+      sized(std::true_type());
+    else
+      sized(std::false_type());
+    src = dst;
   }
+  const uint2* pair = static_cast<const uint2*>(src);
   return with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     constexpr int E = 16 / sizeof(T);
@@ -357,14 +463,21 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
     const int lanes = group_lanes((int)D, wide ? E : 1), cols = lanes * (wide ? E : 1);
     const long long chunks = (N + L - 1) / L;
     const dim3 grid((unsigned)((chunks + kThreads / lanes - 1) / (kThreads / lanes)), (unsigned)((D + cols - 1) / cols));
+    auto go = [&](auto el) {
+      launch(k_embed_sum<T, decltype(el)::value>, grid, kThreads, 0, s, (const T*)g, (int)ldg, pair, (int)N, (unsigned)V,
+             (int)D, L, lanes, (float)scale, (T*)grad, w.part);
+    };
     if (wide)
-      launch(k_embed_sum<T, E>, grid, kThreads, 0, s, (const T*)g, ldg, w.key[at], w.pos[at], N, (unsigned)V, (int)D, L,
-             lanes, (float)scale, (T*)grad, w.part);
+      go(std::integral_constant<int, E>());
     else
-      launch(k_embed_sum<T, 1>, grid, kThreads, 0, s, (const T*)g, ldg, w.key[at], w.pos[at], N, (unsigned)V, (int)D, L,
-             lanes, (float)scale, (T*)grad, w.part);
-    launch(k_embed_join<T>, dim3((unsigned)chunks), kThreads, 0, s, w.key[at], N, (unsigned)V, (int)D, L, (float)scale,
-           w.part, (T*)grad);
+      go(std::integral_constant<int, 1>());
+    if (chunks > 1)
+      launch(k_embed_join<T>, dim3((unsigned)((chunks + 7) / 8)), kThreads, 0, s, pair, (int)N, (unsigned)V, (int)D, L,
+             (unsigned)chunks, (float)scale, w.part, (T*)grad, list_n, w.list);
+    if (chunks > kJoin)
+      launch(k_embed_join_long<T>, dim3((unsigned)(chunks / kJoin < 148 ? chunks / kJoin : 148),
+                                        (unsigned)(D < 256 ? (D + 31) / 32 : 8)),
+             kLongThreads, 0, s, pair, (int)D, L, (unsigned)chunks, (float)scale, w.part, (T*)grad, list_n, w.list);
     return launch_status("embedding_bwd");
   });
 }

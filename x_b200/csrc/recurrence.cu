@@ -228,13 +228,32 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
 }
 
 // ------------------------------------------------------------------------------------------------ between the chunks
-// state[k]: what enters chunk k along the walk.  Per column kChainSegs threads each join a run of chunks, the runs are
-// joined in order, and every thread walks its run again from the true state.
+// state[k]: what enters chunk k along the walk.  Per column kChainSegs threads each join a run of chunks; the runs are
+// joined four to a warp, the warps' eight to a thread of the first warp, and every thread walks its run again from the
+// true state.
+__device__ __forceinline__ Map map_above(const Map& m, int by) {
+  return Map{__shfl_up_sync(0xffffffffu, m.A, by), __shfl_up_sync(0xffffffffu, m.C, by),
+             (bool)__shfl_up_sync(0xffffffffu, (int)m.cut, by)};
+}
+// The map of the runs before this thread's in its warp (lanes of one column are kChainCols apart); m becomes the map up
+// to its own.
+__device__ __forceinline__ Map warp_join(Map& m, int lane) {
+#pragma unroll
+  for (int by = kChainCols; by < 32; by *= 2) {
+    const Map p = map_above(m, by);
+    if (lane >= by) m = then(p, m);
+  }
+  const Map before = map_above(m, kChainCols);
+  return lane < kChainCols ? identity() : before;
+}
+
 template <bool BWD>
 __global__ void __launch_bounds__(kChainCols * kChainSegs) k_rec_chain(const uint2* __restrict__ chunk, int chunks, int D,
                                                                        float* __restrict__ state) {
-  __shared__ uint2 sm[kChainSegs][kChainCols];
-  __shared__ float in[kChainSegs][kChainCols];
+  constexpr int kWarps = kChainCols * kChainSegs / 32, kEach = kWarps * kChainCols / 32;
+  __shared__ uint2 sm[kWarps][kChainCols];
+  __shared__ float in[kWarps][kChainCols];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int x = threadIdx.x % kChainCols, sg = threadIdx.x / kChainCols, c = blockIdx.x * kChainCols + x;
   const int run = (chunks + kChainSegs - 1) / kChainSegs, k0 = sg * run, k1 = min(k0 + run, chunks);
   auto at = [&](int k) { return (long long)(BWD ? chunks - 1 - k : k) * D + c; };
@@ -243,19 +262,24 @@ __global__ void __launch_bounds__(kChainCols * kChainSegs) k_rec_chain(const uin
 #pragma unroll 8
     for (int k = k0; k < k1; ++k) m = then(m, unpack_map(chunk[at(k)]));
   }
-  sm[sg][x] = pack_map(m);
+  const Map before = warp_join(m, lane);
+  if (lane >= 32 - kChainCols) sm[wid][x] = pack_map(m);
   __syncthreads();
-  if (threadIdx.x < kChainCols) {
-    float s = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < kChainSegs; ++k) {
-      in[k][threadIdx.x] = s;
-      s = apply(unpack_map(sm[k][threadIdx.x]), s);
+  if (wid == 0) {
+    const int w0 = lane / kChainCols * kEach;
+    Map t = identity();
+#pragma unroll
+    for (int w = 0; w < kEach; ++w) t = then(t, unpack_map(sm[w0 + w][x]));
+    float s = apply(warp_join(t, lane), 0.f);
+#pragma unroll
+    for (int w = 0; w < kEach; ++w) {
+      in[w0 + w][x] = s;
+      s = apply(unpack_map(sm[w0 + w][x]), s);
     }
   }
   __syncthreads();
   if (c >= D) return;
-  float s = in[sg][x];
+  float s = apply(before, in[wid][x]);
 #pragma unroll 8
   for (int k = k0; k < k1; ++k) {
     const uint2 v = chunk[at(k)];

@@ -26,13 +26,13 @@ __host__ __device__ __forceinline__ void mulhilo32(unsigned a, unsigned b, unsig
   *lo = (unsigned)p;
 }
 
+constexpr unsigned kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u;  // round multipliers
 constexpr unsigned kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;  // key increments (golden ratio, sqrt(3) - 1)
 
 __host__ __device__ __forceinline__ Philox4 philox_round(const Philox4& c, unsigned k0, unsigned k1) {
-  constexpr unsigned kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u;  // round multipliers
   unsigned hi0, lo0, hi1, lo1;
-  mulhilo32(kM0, c.x, &hi0, &lo0);
-  mulhilo32(kM1, c.z, &hi1, &lo1);
+  mulhilo32(kPhiloxM0, c.x, &hi0, &lo0);
+  mulhilo32(kPhiloxM1, c.z, &hi1, &lo1);
   return Philox4{hi1 ^ c.y ^ k0, lo1, hi0 ^ c.w ^ k1, lo0};
 }
 

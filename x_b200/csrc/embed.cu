@@ -14,48 +14,47 @@ namespace {
 constexpr int kThreads = 256;
 
 // ------------------------------------------------------------------------------------------------ forward
-// A group of `lanes` threads (a power of two up to 32) walks kRowsEach rows, E neighbouring columns per thread: the
-// rows' numbers, then all their loads, then the stores.
+// A group of `lanes` threads (up to 32) takes kRowsEach rows, E neighbouring columns per thread: the rows' numbers, then
+// all their loads, then the stores.  Groups need not divide a warp: rows of 96 fp16 columns take 12 threads.
 constexpr int kRowsEach = 4;
 
 template <typename T, int E>
 __global__ void __launch_bounds__(kThreads, 5) k_embed_fwd(const T* __restrict__ W, int ldw, int V, int D,
                                                            const long long* __restrict__ idx, int N, float scale,
                                                            int lanes, T* __restrict__ out) {
-  const int sub = threadIdx.x & (lanes - 1), per = kThreads / lanes;
-  const unsigned n0 = blockIdx.x * (unsigned)(per * kRowsEach) + threadIdx.x / lanes;
+  const int per = kThreads / lanes, mine = threadIdx.x / lanes, c = (blockIdx.y * lanes + threadIdx.x % lanes) * E;
+  if (mine >= per || c >= D) return;
+  const unsigned n = blockIdx.x * (unsigned)(per * kRowsEach) + mine;
   int v[kRowsEach];  // -1: no row
 #pragma unroll
   for (int k = 0; k < kRowsEach; ++k) {
-    const long long i = n0 + k * per < N ? __ldg(idx + n0 + k * per) : -1;
+    const long long i = n + k * per < N ? __ldg(idx + n + k * per) : -1;
     v[k] = i >= 0 && i < V ? (int)i : -1;
   }
-  for (int c = (blockIdx.y * lanes + sub) * E; c < D; c += gridDim.y * lanes * E) {
-    Pack<T, E> r[kRowsEach];
+  Pack<T, E> r[kRowsEach];
 #pragma unroll
-    for (int k = 0; k < kRowsEach; ++k) {
-      if (v[k] >= 0) {
-        r[k] = load_pack<T, E>(W + (long long)v[k] * ldw + c);
-      } else {
+  for (int k = 0; k < kRowsEach; ++k) {
+    if (v[k] >= 0) {
+      r[k] = load_pack<T, E>(W + (long long)v[k] * ldw + c);
+    } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) r[k].v[e] = from_f32<T>(0.f);
-      }
+      for (int e = 0; e < E; ++e) r[k].v[e] = from_f32<T>(0.f);
     }
+  }
 #pragma unroll
-    for (int k = 0; k < kRowsEach; ++k) {
-      // a row outside the table stays zero whatever the scale
-      if (v[k] >= 0) {
+  for (int k = 0; k < kRowsEach; ++k) {
+    if (n + k * per >= N) break;
+    if (v[k] >= 0) {  // a row outside the table stays zero whatever the scale
 #pragma unroll
-        for (int e = 0; e < E; ++e) r[k].v[e] = from_f32<T>(to_f32(r[k].v[e]) * scale);
-      }
-      if (n0 + k * per < N) store_pack(out + (long long)(n0 + k * per) * D + c, r[k]);
+      for (int e = 0; e < E; ++e) r[k].v[e] = from_f32<T>(to_f32(r[k].v[e]) * scale);
     }
+    store_pack(out + (long long)(n + k * per) * D + c, r[k]);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ sort
 // Least-significant-digit radix sort of (row, event) pairs, up to kMaxBits per pass.  A tile is 512 * ITEMS
-// neighbouring pairs; every pass counts the tile's digits, scans the counts (digit-major) and places the pairs.  Tiles
+// neighbouring pairs; every pass counts the tiles' digits, scans the counts and places the pairs.  Tiles
 // of 4096 pairs spread the work per digit (a place per warp and digit to clear and to sum) over more pairs; below 64 tiles
 // of that size the GPU would idle, and tiles of 2048 are taken.
 constexpr int kSortThreads = 512;
@@ -81,8 +80,7 @@ __device__ __forceinline__ Pair sort_pair(const void* src, long long i, unsigned
 
 template <bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) k_sort_count(const void* __restrict__ src, long long N, unsigned V,
-                                                             int shift, int bins, int tiles,
-                                                             unsigned* __restrict__ counts,
+                                                             int shift, int bins, unsigned* __restrict__ counts,
                                                              unsigned* __restrict__ list_n) {
   __shared__ unsigned hist[kMaxBins];
   if (blockIdx.x == 0 && threadIdx.x == 0) *list_n = 0;  // for the kernels behind the sort
@@ -95,7 +93,7 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_count(const void* __restr
     if (i < N) atomicAdd(&hist[(sort_pair<FIRST>(src, i, V).row >> shift) & (bins - 1)], 1u);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) counts[(long long)d * tiles + blockIdx.x] = hist[d];
+  for (int d = threadIdx.x; d < bins; d += kSortThreads) counts[(long long)blockIdx.x * bins + d] = hist[d];
 }
 
 // Exclusive sum over the CTA's THREADS threads; returns this thread's, *total the whole.
@@ -121,36 +119,56 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* sm, unsigne
   return before + inc - v;
 }
 
-// One CTA per digit: its counts over the tiles become offsets within the digit.
-__global__ void __launch_bounds__(kThreads) k_sort_scan(unsigned* __restrict__ counts, int tiles,
-                                                        unsigned* __restrict__ totals) {
-  __shared__ unsigned sm[kThreads / 32];
-  unsigned* row = counts + (long long)blockIdx.x * tiles;
-  unsigned carry = 0;
-  for (int t0 = 0; t0 < tiles; t0 += kThreads) {
-    const int t = t0 + threadIdx.x;
-    const unsigned v = t < tiles ? row[t] : 0;
-    unsigned total;
-    const unsigned ex = block_scan<kThreads>(v, sm, &total);
-    if (t < tiles) row[t] = carry + ex;
-    carry += total;
+// A CTA per 32 digits: their counts over the tiles become offsets within the digit.  A thread sums a run of tiles, the
+// 32 runs of a digit are joined, and the thread walks its run again.
+__global__ void __launch_bounds__(1024) k_sort_scan(unsigned* __restrict__ counts, int bins, int tiles,
+                                                    unsigned* __restrict__ totals) {
+  __shared__ unsigned sm[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, d = blockIdx.x * 32 + x;
+  const int run = (tiles + 31) / 32, t0 = y * run, t1 = min(t0 + run, tiles);
+  unsigned sum = 0;
+  if (d < bins) {
+#pragma unroll 8
+    for (int t = t0; t < t1; ++t) sum += counts[(long long)t * bins + d];
   }
-  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+  sm[y][x] = sum;
+  __syncthreads();
+  // the warp of digit row y joins the 32 runs of digit y
+  unsigned inc = sm[x][y];
+  const unsigned own = inc;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (x >= o) inc += u;
+  }
+  sm[x][y] = inc - own;
+  if (x == 31 && blockIdx.x * 32 + y < bins) totals[blockIdx.x * 32 + y] = inc;
+  __syncthreads();
+  if (d >= bins) return;
+  unsigned at = sm[y][x];
+#pragma unroll 8
+  for (int t = t0; t < t1; ++t) {
+    const unsigned c = counts[(long long)t * bins + d];
+    counts[(long long)t * bins + d] = at;
+    at += c;
+  }
 }
 
 // Stable placement: a warp ranks 32 neighbouring pairs at a time among equal digits (match), on top of the counts
-// of the rounds and warps before it.
+// of the rounds and warps before it.  The tile is put in order in shared memory first, so that pairs of one digit leave
+// side by side: scattered one by one, 1M pairs take 19 us a pass.
 template <bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restrict__ src, long long N, unsigned V,
-                                                             int shift, int bins, int tiles,
-                                                             const unsigned* __restrict__ counts,
+                                                             int shift, int bins, const unsigned* __restrict__ counts,
                                                              const unsigned* __restrict__ totals,
                                                              uint2* __restrict__ out) {
-  __shared__ unsigned short hist[kSortWarps][kMaxBins];
-  __shared__ unsigned start[kMaxBins];
+  constexpr int kTile = kSortThreads * ITEMS;
+  static_assert(kTile * sizeof(uint2) <= sizeof(unsigned short) * kSortWarps * kMaxBins, "the pairs reuse the counts");
+  __shared__ __align__(8) unsigned short hist[kSortWarps][kMaxBins];
+  __shared__ unsigned start[kMaxBins], local[kMaxBins];
   __shared__ unsigned sm[kSortWarps];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const long long base = blockIdx.x * (long long)(kSortThreads * ITEMS) + wid * (32 * ITEMS) + lane;
+  const long long tile0 = blockIdx.x * (long long)kTile, base = tile0 + wid * (32 * ITEMS) + lane;
   Pair p[ITEMS];
 #pragma unroll
   for (int r = 0; r < ITEMS; ++r)
@@ -161,10 +179,10 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restr
     const int d = d0 + threadIdx.x;
     unsigned total;
     const unsigned ex = block_scan<kSortThreads>(d < bins ? totals[d] : 0, sm, &total);
-    if (d < bins) start[d] = carry + ex + counts[(long long)d * tiles + blockIdx.x];
+    if (d < bins) start[d] = carry + ex + counts[(long long)blockIdx.x * bins + d];
     carry += total;
   }
-  unsigned rank[ITEMS];
+  unsigned at[ITEMS];  // rank among the warp's pairs of the digit, then the place in the tile
 #pragma unroll
   for (int r = 0; r < ITEMS; ++r) {
     const bool in = base + r * 32 < N;
@@ -173,26 +191,51 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restr
     unsigned before = 0;
     if (in) before = hist[wid][d];
     __syncwarp();
-    rank[r] = before + __popc(peers & ((1u << lane) - 1));
+    at[r] = before + __popc(peers & ((1u << lane) - 1));
     if (in && lane == __ffs(peers) - 1) hist[wid][d] = (unsigned short)(before + __popc(peers));
     __syncwarp();
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) {
-    unsigned c = 0;
+  carry = 0;
+  for (int d0 = 0; d0 < bins; d0 += kSortThreads) {
+    const int d = d0 + threadIdx.x;
+    unsigned c = 0, total;
+    if (d < bins) {
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
-      const unsigned h = hist[w][d];
-      hist[w][d] = (unsigned short)c;
-      c += h;
+      for (int w = 0; w < kSortWarps; ++w) {
+        const unsigned h = hist[w][d];
+        hist[w][d] = (unsigned short)c;
+        c += h;
+      }
     }
+    const unsigned ex = block_scan<kSortThreads>(c, sm, &total);
+    if (d < bins) {
+      local[d] = carry + ex;
+      start[d] -= carry + ex;
+    }
+    carry += total;
   }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < ITEMS; ++r) {
     if (base + r * 32 < N) {
       const unsigned d = (p[r].row >> shift) & (bins - 1);
-      out[start[d] + hist[wid][d] + rank[r]] = make_uint2(p[r].row, p[r].event);
+      at[r] += local[d] + hist[wid][d];
+    }
+  }
+  __syncthreads();
+  uint2* tile = reinterpret_cast<uint2*>(hist);
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r)
+    if (base + r * 32 < N) tile[at[r]] = make_uint2(p[r].row, p[r].event);
+  __syncthreads();
+  const int n = N - tile0 < kTile ? (int)(N - tile0) : kTile;
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    const int i = r * kSortThreads + threadIdx.x;
+    if (i < n) {
+      const uint2 q = tile[i];
+      out[start[(q.x >> shift) & (bins - 1)] + i] = q;
     }
   }
 }
@@ -225,10 +268,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_embed_sum(const T* __restrict__
                                                            const uint2* __restrict__ pair, int N, unsigned V, int D,
                                                            int L, int lanes, float scale, T* __restrict__ grad,
                                                            float* __restrict__ part) {
-  const int sub = threadIdx.x & (lanes - 1), per = kThreads / lanes;
-  const unsigned chunk = blockIdx.x * (unsigned)per + threadIdx.x / lanes;
-  const int c = (blockIdx.y * lanes + sub) * E;
-  if ((long long)chunk * L >= N || c >= D) return;
+  const int per = kThreads / lanes, mine = threadIdx.x / lanes, c = (blockIdx.y * lanes + threadIdx.x % lanes) * E;
+  const unsigned chunk = blockIdx.x * (unsigned)per + mine;
+  if (mine >= per || (long long)chunk * L >= N || c >= D) return;
   const int j0 = chunk * L, j1 = min(N - j0, L) + j0;
   const unsigned prev = j0 > 0 ? pair[j0 - 1].x : 0xffffffffu;
   unsigned cur = pair[j0].x;
@@ -248,21 +290,27 @@ __global__ void __launch_bounds__(kThreads, 4) k_embed_sum(const T* __restrict__
       store_pack(grad + (long long)cur * D + c, r);
     }
   };
+  uint2 next[kAhead];  // the pairs of the next rows, on the way while these rows are summed
+#pragma unroll
+  for (int q = 0; q < kAhead; ++q) next[q] = j0 + q < j1 ? __ldg(pair + j0 + q) : make_uint2(V, 0);
 #pragma unroll 1
   for (int j = j0; j < j1 && cur < V; j += kAhead) {
     unsigned row[kAhead];
     Pack<T, E> r[kAhead];
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
-      uint2 k = make_uint2(V, 0);
-      if (j + q < j1) k = __ldg(pair + j + q);
-      row[q] = k.x;
-      if (k.x < V) {
-        r[q] = load_pack<T, E>(g + (long long)k.y * ldg + c);
+      row[q] = next[q].x;
+      if (row[q] < V) {
+        r[q] = load_pack<T, E>(g + (long long)next[q].y * ldg + c);
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) r[q].v[e] = from_f32<T>(0.f);
       }
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int m = j + kAhead + q;
+      next[q] = m < j1 ? __ldg(pair + m) : make_uint2(V, 0);
     }
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
@@ -298,9 +346,8 @@ __global__ void __launch_bounds__(kThreads) k_embed_join(const uint2* __restrict
   const int lane = threadIdx.x & 31;
   if (chunk + 1 >= chunks) return;
   const int j0 = chunk * L, j1 = j0 + L;
-  const unsigned cur = pair[j1 - 1].x;
-  if (cur >= V || pair[j1].x != cur) return;
-  if (j0 > 0 && pair[j0].x == cur && pair[j0 - 1].x == cur) return;  // it began further left
+  const unsigned cur = pair[j1 - 1].x, after = pair[j1].x, first = pair[j0].x, before = j0 > 0 ? pair[j0 - 1].x : V;
+  if (cur >= V || after != cur || (first == cur && before == cur)) return;  // none, or it began further left
   // lane i: does the run go on into chunk + 2 + i?
   const unsigned next = chunk + 2 + lane;
   const unsigned stops = __ballot_sync(0xffffffffu, next >= chunks || pair[(long long)next * L].x != cur);
@@ -317,17 +364,17 @@ __global__ void __launch_bounds__(kThreads) k_embed_join(const uint2* __restrict
   }
 }
 
-// Long runs, a CTA for each and 32 columns: 32 warps take every 32nd partial sum each, then their sums are added in
-// order.
-constexpr int kLongThreads = 1024;
+// Long runs, a CTA for each and kLongCols columns: its 64 rows of threads take every 64th partial sum each, then their
+// sums are added in order.
+constexpr int kLongCols = 16, kLongRows = 64, kLongThreads = kLongCols * kLongRows;
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads) k_embed_join_long(const uint2* __restrict__ pair, int D, int L,
                                                                   unsigned chunks, float scale,
                                                                   const float* __restrict__ part, T* __restrict__ grad,
                                                                   const unsigned* __restrict__ list_n,
                                                                   const LongRun* __restrict__ list) {
-  __shared__ float sm[32][33];
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  __shared__ float sm[kLongRows][kLongCols + 1];
+  const int x = threadIdx.x % kLongCols, y = threadIdx.x / kLongCols;
   const unsigned n = *list_n;
   for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
     const LongRun run = list[i];
@@ -339,18 +386,19 @@ __global__ void __launch_bounds__(kLongThreads) k_embed_join_long(const uint2* _
       last += more;
       if (more < kLongThreads) break;
     }
-    for (int c0 = blockIdx.y * 32; c0 < D; c0 += gridDim.y * 32) {
-      const int c = c0 + lane;
+    for (int c0 = blockIdx.y * kLongCols; c0 < D; c0 += gridDim.y * kLongCols) {
+      const int c = c0 + x;
       float acc = 0.f;
       if (c < D) {
-        if (wid == 0) acc = part[((long long)run.chunk * 2 + 1) * D + c];
+        if (y == 0) acc = part[((long long)run.chunk * 2 + 1) * D + c];
 #pragma unroll 8
-        for (unsigned e = run.chunk + 1 + wid; e <= last; e += 32) acc += part[(long long)e * 2 * D + c];
+        for (unsigned e = run.chunk + 1 + y; e <= last; e += kLongRows) acc += part[(long long)e * 2 * D + c];
       }
-      sm[wid][lane] = acc;
+      sm[y][x] = acc;
       __syncthreads();
-      if (wid == 0 && c < D) {
-        for (int w = 1; w < 32; ++w) acc += sm[w][lane];
+      if (y == 0 && c < D) {
+#pragma unroll 8
+        for (int w = 1; w < kLongRows; ++w) acc += sm[w][x];
         grad[(long long)run.row * D + c] = from_f32<T>(acc * scale);
       }
       __syncthreads();
@@ -358,17 +406,14 @@ __global__ void __launch_bounds__(kLongThreads) k_embed_join_long(const uint2* _
   }
 }
 
-// Pairs per chunk: about 16384 chunks where there are enough pairs, one wave of groups on the GPU.
-int sum_chunk(long long N) {
-  int L = 16;
-  while (L < (1 << 20) && N / L > 16384) L *= 2;
-  return L;
-}
+// Threads on a row of D columns, E each.
+int group_lanes(long long D, int E) { return D >= 32LL * E ? 32 : D < 1 ? 1 : (int)((D + E - 1) / E); }
 
-int group_lanes(int D, int E) {
-  int l = 1;
-  while (l < 32 && l * E < D) l *= 2;
-  return l;
+// Pairs per chunk: one wave of groups on the GPU (148 SMs of 4 CTAs, groups of 16-byte threads on 16-bit rows), so that
+// all end together.
+int sum_chunk(long long N, long long D) {
+  const long long wave = 148LL * 4 * (kThreads / group_lanes(D, 8)), L = (N + wave - 1) / wave;
+  return (int)(L < 16 ? 16 : L);
 }
 
 struct EmbedWs {
@@ -381,7 +426,7 @@ struct EmbedWs {
 
 EmbedWs carve(void* ws, long long N, long long V, long long D) {
   const SortPlan s = sort_plan(N, V);
-  const int L = sum_chunk(N);
+  const int L = sum_chunk(N, D);
   Carve c(ws);
   EmbedWs w;
   for (int i = 0; i < 2; ++i) w.pair[i] = c.take<uint2>(s.passes > i ? N : 0);
@@ -404,11 +449,11 @@ int embedding_fwd(int dtype, const void* W, long long ldw, long long V, long lon
     using T = decltype(tag);
     constexpr int E = 16 / sizeof(T);
     const bool wide = D % E == 0 && ldw % E == 0 && aligned_to(W, 16) && aligned_to(out, 16);
-    const int lanes = group_lanes((int)D, wide ? E : 1);
+    const int lanes = group_lanes(D, wide ? E : 1);
+    const int E1 = wide ? E : 1;
     const long long per = kThreads / lanes * kRowsEach;
-    // few rows of many columns: the columns spread over CTAs as well
-    const int E1 = wide ? E : 1, slabs = (int)((D + lanes * E1 - 1) / (lanes * E1));
-    const dim3 grid((unsigned)((N + per - 1) / per), N < per * 148 ? (slabs < 65535 ? slabs : 65535) : 1);
+    const unsigned slabs = (unsigned)((D + lanes * E1 - 1) / (lanes * E1));
+        const dim3 grid((unsigned)((N + per - 1) / per), slabs);
     auto go = [&](auto el) {
       launch(k_embed_fwd<T, decltype(el)::value>, grid, kThreads, 0, s, (const T*)W, (int)ldw, (int)V, (int)D, idx, (int)N,
              (float)scale, lanes, (T*)out);
@@ -429,7 +474,7 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
   if (N <= 0) return ATLB_OK;
   const SortPlan p = sort_plan(N, V);
   const EmbedWs w = carve(ws, N, V, D);
-  const int bins = 1 << p.bits, L = sum_chunk(N);
+  const int bins = 1 << p.bits, L = sum_chunk(N, D);
   unsigned* list_n = w.totals + bins;
   const void* src = idx;
   for (int i = 0; i < p.passes; ++i) {
@@ -437,11 +482,10 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
     auto pass = [&](auto first, auto items) {
       constexpr bool F = decltype(first)::value;
       constexpr int I = decltype(items)::value;
-      launch(k_sort_count<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, p.tiles, w.counts,
-             list_n);
-      launch(k_sort_scan, bins, kThreads, 0, s, w.counts, p.tiles, w.totals);
-      launch(k_sort_place<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, p.tiles, w.counts,
-             w.totals, dst);
+      launch(k_sort_count<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, w.counts, list_n);
+      launch(k_sort_scan, (bins + 31) / 32, 1024, 0, s, w.counts, bins, p.tiles, w.totals);
+      launch(k_sort_place<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, w.counts, w.totals,
+             dst);
     };
     auto sized = [&](auto first) {
       if (p.large)
@@ -460,7 +504,7 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
     using T = decltype(tag);
     constexpr int E = 16 / sizeof(T);
     const bool wide = D % E == 0 && ldg % E == 0 && aligned_to(g, 16) && aligned_to(grad, 16);
-    const int lanes = group_lanes((int)D, wide ? E : 1), cols = lanes * (wide ? E : 1);
+    const int lanes = group_lanes(D, wide ? E : 1), cols = lanes * (wide ? E : 1);
     const long long chunks = (N + L - 1) / L;
     const dim3 grid((unsigned)((chunks + kThreads / lanes - 1) / (kThreads / lanes)), (unsigned)((D + cols - 1) / cols));
     auto go = [&](auto el) {
@@ -476,7 +520,7 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
              (unsigned)chunks, (float)scale, w.part, (T*)grad, list_n, w.list);
     if (chunks > kJoin)
       launch(k_embed_join_long<T>, dim3((unsigned)(chunks / kJoin < 148 ? chunks / kJoin : 148),
-                                        (unsigned)(D < 256 ? (D + 31) / 32 : 8)),
+                                        (unsigned)(D < 256 ? (D + kLongCols - 1) / kLongCols : 16)),
              kLongThreads, 0, s, pair, (int)D, L, (unsigned)chunks, (float)scale, w.part, (T*)grad, list_n, w.list);
     return launch_status("embedding_bwd");
   });

@@ -23,7 +23,14 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kGroup = 32;          // rows of a group
 constexpr int kPart = 8;                      // rows between the states that the forward pass keeps for the backward pass
-constexpr int kBytes = 8;           // of a row per thread, where the rows are whole multiples of it
+#ifndef RB_M
+#define RB_M 5
+#define RB_F 5
+#define RB_B 3
+#define RB_BYTES 8
+#define RB_AHEAD 4
+#endif
+constexpr int kBytes = RB_BYTES;           // of a row per thread, where the rows are whole multiples of it
 constexpr int kSeg = 16;            // groups joined by one thread
 constexpr int kChainCols = 8, kChainSegs = 128;
 
@@ -40,11 +47,10 @@ struct RecShape {
 // a = 1 / (1 + exp(-z)) and 1 - a = exp(-z) a.  The exponent is capped so that exp(-z) stays finite: below -87 a is
 // held at 2^-126, where fp32's normal numbers end.
 __device__ __forceinline__ void sigmoid2(float z, float* a, float* w) {
-  float e, r;
-  const float t = fminf(z * -1.44269504f, 126.f);
+  float t, e;
+  asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(t) : "f"(z * -1.44269504f));  // 126; a NaN stays one
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  *a = z == z ? r : z;  // fminf passes a NaN over
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(*a) : "f"(1.f + e));
   *w = e * *a;
 }
 
@@ -145,10 +151,10 @@ struct Src {
 // Threads `lanes` wide on a row, E neighbouring columns each; the CTA's groups are one chunk.  BWD walks from the last
 // row to the first: in = dL/dh, and the state is u.  prefix: the map from the chunk's entry to the group's; chunk: the
 // whole chunk's map.
-constexpr int kAhead = 4;  // rows in flight per thread
+constexpr int kAhead = RB_AHEAD;  // rows in flight per thread
 
 template <typename T, int E, int KIND, bool BWD>
-__global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate, Src<T> in, const float* __restrict__ s0,
+__global__ void __launch_bounds__(kThreads, RB_M) k_rec_map(RecShape S, Src<T> gate, Src<T> in, const float* __restrict__ s0,
                                                       uint2* __restrict__ prefix, uint2* __restrict__ chunk) {
   __shared__ uint2 sm[kThreads * E];
   __shared__ uint2 seg[32 * E];  // segments x columns: 16 E, or 32 E where a warp takes a row
@@ -162,15 +168,21 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
 #pragma unroll
   for (int e = 0; e < E; ++e) { A[e] = 1.f; s[e] = 0.f; }
   auto rows = [&](auto plain) {
+    // rows are stepped through by pointer: a product with the stride per row costs as much as four additions.  Threads
+    // behind the last column read the first and are not heard.
+    const long long dg = BWD ? -gate.ld : gate.ld, di = BWD ? -in.ld : in.ld, from = r0 + (BWD ? kGroup - 1 : 0);
+    const T *pg = gate.p + from * gate.ld + (col ? c : 0), *pi = in.p + from * in.ld + (col ? c : 0);
 #pragma unroll 1
     for (int q = 0; q < kGroup; q += kAhead) {
       Pack<T, E> gp[kAhead], ip[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int r = BWD ? kGroup - 1 - q - j : q + j;
-        const bool ok = col && (decltype(plain)::value || !(ed.none >> r & 1));
-        gp[j] = load_or_zero<T, E>(gate.p + (r0 + r) * gate.ld + c, ok);
-        ip[j] = load_or_zero<T, E>(in.p + (r0 + r) * in.ld + c, ok);
+        const bool ok = decltype(plain)::value || !(ed.none >> r & 1);
+        gp[j] = load_or_zero<T, E>(pg, ok);
+        ip[j] = load_or_zero<T, E>(pi, ok);
+        pg += dg;
+        pi += di;
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
@@ -302,7 +314,7 @@ __device__ __forceinline__ void group_state(const RecShape& S, const uint2* pref
 
 // ------------------------------------------------------------------------------------------------ replay, forward
 template <typename T, int E, int KIND>
-__global__ void __launch_bounds__(kThreads, 4) k_rec_fwd(RecShape S, Src<T> gate, Src<T> x, const float* __restrict__ h0,
+__global__ void __launch_bounds__(kThreads, RB_F) k_rec_fwd(RecShape S, Src<T> gate, Src<T> x, const float* __restrict__ h0,
                                                       const uint2* __restrict__ prefix,
                                                       const float* __restrict__ state, T* __restrict__ h,
                                                       float* __restrict__ hT, float* __restrict__ saved) {
@@ -316,14 +328,18 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_fwd(RecShape S, Src<T> gate
   float s[E];
   group_state(S, prefix, state, g, per, c, col && g < S.groups, s);
   auto rows = [&](auto plain) {
+    const T *pg = gate.p + r0 * gate.ld + (col ? c : 0), *px = x.p + r0 * x.ld + (col ? c : 0);
+    T* ph = h + r0 * S.D + c;
 #pragma unroll 1
     for (int q = 0; q < kGroup; q += kAhead) {
       Pack<T, E> gp[kAhead], xp[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const bool ok = col && (decltype(plain)::value || !(ed.none >> (q + j) & 1));
-        gp[j] = load_or_zero<T, E>(gate.p + (r0 + q + j) * gate.ld + c, ok);
-        xp[j] = load_or_zero<T, E>(x.p + (r0 + q + j) * x.ld + c, ok);
+        const bool ok = decltype(plain)::value || !(ed.none >> (q + j) & 1);
+        gp[j] = load_or_zero<T, E>(pg, ok);
+        xp[j] = load_or_zero<T, E>(px, ok);
+        pg += gate.ld;
+        px += x.ld;
       }
       if (saved && q % kPart == 0 && col && r0 + q < S.N) {
 #pragma unroll
@@ -344,7 +360,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_fwd(RecShape S, Src<T> gate
           s[e] = fmaf(a, s[e], v);
           o.v[e] = from_f32<T>(s[e]);
         }
-        if (col && (decltype(plain)::value || r0 + r < S.N)) store_pack(h + (r0 + r) * S.D + c, o);
+        if (col && (decltype(plain)::value || r0 + r < S.N)) store_pack(ph, o);
+        ph += S.D;
         if (!decltype(plain)::value && hT && col && (ed.last & ~ed.none) >> r & 1) {
           const int win = window_of(S, r0 + r);
 #pragma unroll
@@ -363,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_fwd(RecShape S, Src<T> gate
 // lanes_b threads on a row, E columns each (4 bytes), a group per `lanes_b` threads.  Each part of the group, the last
 // one first: its rows in registers, the states forward from the one the forward pass kept, then u backward.
 template <typename T, int E, int KIND>
-__global__ void __launch_bounds__(kThreads, 4) k_rec_bwd(RecShape S, int lanes_b, Src<T> gate, Src<T> x, Src<T> gh,
+__global__ void __launch_bounds__(kThreads, RB_B) k_rec_bwd(RecShape S, int lanes_b, Src<T> gate, Src<T> x, Src<T> gh,
                                                          const float* __restrict__ h0, const float* __restrict__ ghT,
                                                          const float* __restrict__ saved,
                                                          const uint2* __restrict__ prefix,
@@ -379,14 +396,21 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_bwd(RecShape S, int lanes_b
   float u[E];
   group_state(S, prefix, state, g, kThreads / S.lanes, c, col && g < S.groups, u);
   auto part = [&](int lo, auto plain) {
-    Pack<T, E> gp[kPart], xp[kPart], dp[kPart];
-    float hp[kPart][E], s[E];
+    Pack<T, E> xp[kPart], dp[kPart];
+    float a[kPart][E], w[kPart][E], hp[kPart][E], s[E];
+    const int cc = col ? c : 0;
+    const T *pg = gate.p + (r0 + lo) * gate.ld + cc, *px = x.p + (r0 + lo) * x.ld + cc,
+            *pd = gh.p + (r0 + lo) * gh.ld + cc;
+    Pack<T, E> gp[kPart];
 #pragma unroll
     for (int r = 0; r < kPart; ++r) {
-      const bool ok = col && (decltype(plain)::value || !(ed.none >> (lo + r) & 1));
-      gp[r] = load_or_zero<T, E>(gate.p + (r0 + lo + r) * gate.ld + c, ok);
-      xp[r] = load_or_zero<T, E>(x.p + (r0 + lo + r) * x.ld + c, ok);
-      dp[r] = load_or_zero<T, E>(gh.p + (r0 + lo + r) * gh.ld + c, ok);
+      const bool ok = decltype(plain)::value || !(ed.none >> (lo + r) & 1);
+      gp[r] = load_or_zero<T, E>(pg, ok);
+      xp[r] = load_or_zero<T, E>(px, ok);
+      dp[r] = load_or_zero<T, E>(pd, ok);
+      pg += gate.ld;
+      px += x.ld;
+      pd += gh.ld;
     }
     load_state(saved, (r0 + lo) / kPart, S.D, c, col && r0 + lo < S.N, s);
 #pragma unroll
@@ -397,12 +421,14 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_bwd(RecShape S, int lanes_b
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        float a, w, v;
-        row_terms<KIND>(to_f32(gp[r].v[e]), to_f32(xp[r].v[e]), &a, &w, &v);
-        hp[r][e] = s[e];
-        s[e] = fmaf(a, s[e], v);
+        float v;
+        const float xv = to_f32(xp[r].v[e]);
+        row_terms<KIND>(to_f32(gp[r].v[e]), xv, &a[r][e], &w[r][e], &v);
+        hp[r][e] = KIND == ATLB_REC_SIGMOID ? w[r][e] * (s[e] - xv) : s[e];  // what the gate's gradient takes
+        s[e] = fmaf(a[r][e], s[e], v);
       }
     }
+    long long at = (r0 + lo + kPart - 1) * S.D + c;
 #pragma unroll
     for (int r = kPart - 1; r >= 0; --r) {
       if (!decltype(plain)::value && (edge_u >> (lo + r) & 1)) {
@@ -412,17 +438,16 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_bwd(RecShape S, int lanes_b
       Pack<T, E> og, ox;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        float a, w, v;
-        const float xv = to_f32(xp[r].v[e]), gt = to_f32(dp[r].v[e]) + u[e];
-        row_terms<KIND>(to_f32(gp[r].v[e]), xv, &a, &w, &v);
-        u[e] = a * gt;
-        og.v[e] = from_f32<T>(KIND == ATLB_REC_SIGMOID ? u[e] * (w * (hp[r][e] - xv)) : gt * hp[r][e]);
-        ox.v[e] = from_f32<T>(KIND == ATLB_REC_SIGMOID ? gt * w : gt);
+        const float gt = to_f32(dp[r].v[e]) + u[e];
+        u[e] = a[r][e] * gt;
+        og.v[e] = from_f32<T>(KIND == ATLB_REC_SIGMOID ? u[e] * hp[r][e] : gt * hp[r][e]);
+        ox.v[e] = from_f32<T>(KIND == ATLB_REC_SIGMOID ? gt * w[r][e] : gt);
       }
       if (col && (decltype(plain)::value || r0 + lo + r < S.N)) {
-        store_pack(ggate + (r0 + lo + r) * S.D + c, og);
-        store_pack(gx + (r0 + lo + r) * S.D + c, ox);
+        store_pack(ggate + at, og);
+        store_pack(gx + at, ox);
       }
+      at -= S.D;
       if (!decltype(plain)::value && gh0 && col && (ed.first & ~ed.none) >> (lo + r) & 1) {
         const int win = window_of(S, r0 + lo + r);
 #pragma unroll

@@ -80,10 +80,22 @@ __device__ __forceinline__ Pair sort_pair(const void* src, long long i, unsigned
 
 template <bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) k_sort_count(const void* __restrict__ src, long long N, unsigned V,
-                                                             int shift, int bins, unsigned* __restrict__ counts,
-                                                             unsigned* __restrict__ list_n) {
+                                                             int shift, int bins, int tiles,
+                                                             unsigned* __restrict__ counts, char* __restrict__ grad,
+                                                             long long grad_bytes) {
   __shared__ unsigned hist[kMaxBins];
-  if (blockIdx.x == 0 && threadIdx.x == 0) *list_n = 0;  // for the kernels behind the sort
+  // on the way, and in CTAs of their own behind the tiles: the gradient starts as zeros (rows that no pair names)
+  if (FIRST) {
+    const long long vecs = grad_bytes / 16, step = (long long)gridDim.x * kSortThreads;
+    const long long i0 = blockIdx.x * (long long)kSortThreads + threadIdx.x;
+    if (reinterpret_cast<uintptr_t>(grad) % 16 == 0) {
+      for (long long i = i0; i < vecs; i += step) reinterpret_cast<uint4*>(grad)[i] = make_uint4(0, 0, 0, 0);
+      if (i0 < grad_bytes % 16) grad[vecs * 16 + i0] = 0;
+    } else {
+      for (long long i = i0; i < grad_bytes / 2; i += step) reinterpret_cast<unsigned short*>(grad)[i] = 0;
+    }
+  }
+  if (blockIdx.x >= tiles) return;
   for (int d = threadIdx.x; d < bins; d += kSortThreads) hist[d] = 0;
   __syncthreads();
   const long long base = blockIdx.x * (long long)(kSortThreads * ITEMS);
@@ -182,14 +194,15 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restr
     if (d < bins) start[d] = carry + ex + counts[(long long)blockIdx.x * bins + d];
     carry += total;
   }
-  unsigned at[ITEMS];  // rank among the warp's pairs of the digit, then the place in the tile
+  unsigned at[ITEMS];  // lanes of the same digit, then the rank among the warp's pairs of it, then the place in the tile
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r)
+    at[r] = __match_any_sync(0xffffffffu, base + r * 32 < N ? (p[r].row >> shift) & (bins - 1) : 0xffffffffu);
 #pragma unroll
   for (int r = 0; r < ITEMS; ++r) {
     const bool in = base + r * 32 < N;
-    const unsigned d = in ? (p[r].row >> shift) & (bins - 1) : 0xffffffffu;
-    const unsigned peers = __match_any_sync(0xffffffffu, d);
-    unsigned before = 0;
-    if (in) before = hist[wid][d];
+    const unsigned d = in ? (p[r].row >> shift) & (bins - 1) : 0, peers = at[r];
+    const unsigned before = in ? hist[wid][d] : 0;
     __syncwarp();
     at[r] = before + __popc(peers & ((1u << lane) - 1));
     if (in && lane == __ffs(peers) - 1) hist[wid][d] = (unsigned short)(before + __popc(peers));
@@ -330,76 +343,68 @@ __global__ void __launch_bounds__(kThreads, 4) k_embed_sum(const T* __restrict__
   put(head || on, head ? 0 : 1);
 }
 
-// The chunk in which a run over several chunks begins joins its partial sums, in order: a warp per chunk.  Runs that go
-// on over kJoin chunks or more are put on a list for k_embed_join_long (in any order: each gives its own row).
-constexpr int kJoin = 32;
-struct LongRun {
-  unsigned chunk, row;
-};
+// The chunk in which a run over several chunks begins joins its partial sums.  A CTA looks after 32 chunks: a warp each
+// for the runs that go on over fewer than 32 more chunks, in order; then, for a longer one, all its threads, 64 rows of
+// them over 16 columns: each takes every 64th partial sum, and these are added in order.
+constexpr int kJoinThreads = 1024, kLongCols = 16, kLongRows = kJoinThreads / kLongCols;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_embed_join(const uint2* __restrict__ pair, int N, unsigned V, int D, int L,
-                                                         unsigned chunks, float scale, const float* __restrict__ part,
-                                                         T* __restrict__ grad, unsigned* __restrict__ list_n,
-                                                         LongRun* __restrict__ list) {
-  const unsigned chunk = blockIdx.x * (unsigned)(kThreads / 32) + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31;
-  if (chunk + 1 >= chunks) return;
-  const int j0 = chunk * L, j1 = j0 + L;
-  const unsigned cur = pair[j1 - 1].x, after = pair[j1].x, first = pair[j0].x, before = j0 > 0 ? pair[j0 - 1].x : V;
-  if (cur >= V || after != cur || (first == cur && before == cur)) return;  // none, or it began further left
-  // lane i: does the run go on into chunk + 2 + i?
-  const unsigned next = chunk + 2 + lane;
-  const unsigned stops = __ballot_sync(0xffffffffu, next >= chunks || pair[(long long)next * L].x != cur);
-  if (stops == 0) {
-    if (lane == 0) list[atomicAdd(list_n, 1u)] = LongRun{chunk, cur};
-    return;
-  }
-  const unsigned last = chunk + __ffs(stops);
-  for (int c = lane; c < D; c += 32) {
-    float acc = part[((long long)chunk * 2 + 1) * D + c];
-#pragma unroll 4
-    for (unsigned e = chunk + 1; e <= last; ++e) acc += part[(long long)e * 2 * D + c];
-    grad[(long long)cur * D + c] = from_f32<T>(acc * scale);
-  }
-}
-
-// Long runs, a CTA for each and kLongCols columns: its 64 rows of threads take every 64th partial sum each, then their
-// sums are added in order.
-constexpr int kLongCols = 16, kLongRows = 64, kLongThreads = kLongCols * kLongRows;
-template <typename T>
-__global__ void __launch_bounds__(kLongThreads) k_embed_join_long(const uint2* __restrict__ pair, int D, int L,
-                                                                  unsigned chunks, float scale,
-                                                                  const float* __restrict__ part, T* __restrict__ grad,
-                                                                  const unsigned* __restrict__ list_n,
-                                                                  const LongRun* __restrict__ list) {
+__global__ void __launch_bounds__(kJoinThreads) k_embed_join(const uint2* __restrict__ pair, int N, unsigned V, int D,
+                                                             int L, unsigned chunks, float scale,
+                                                             const float* __restrict__ part, T* __restrict__ grad) {
   __shared__ float sm[kLongRows][kLongCols + 1];
+  __shared__ unsigned long_row[32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const unsigned chunk = blockIdx.x * 32 + wid;
+  unsigned row = V;  // of a run that begins here and goes on
+  if (chunk + 1 < chunks) {
+    const int j0 = chunk * L, j1 = j0 + L;
+    const unsigned cur = pair[j1 - 1].x, after = pair[j1].x, first = pair[j0].x, before = j0 > 0 ? pair[j0 - 1].x : V;
+    if (cur < V && after == cur && !(first == cur && before == cur)) row = cur;
+  }
+  bool is_long = false;
+  if (row < V) {
+    // lane i: does the run end before chunk + 2 + i?
+    const unsigned next = chunk + 2 + lane;
+    const unsigned ends = __ballot_sync(0xffffffffu, next >= chunks || pair[(long long)next * L].x != row);
+    is_long = ends == 0;
+    if (!is_long && blockIdx.y == 0) {
+      const unsigned last = chunk + __ffs(ends);
+      for (int c = lane; c < D; c += 32) {
+        float acc = part[((long long)chunk * 2 + 1) * D + c];
+#pragma unroll 4
+        for (unsigned e = chunk + 1; e <= last; ++e) acc += part[(long long)e * 2 * D + c];
+        grad[(long long)row * D + c] = from_f32<T>(acc * scale);
+      }
+    }
+  }
+  if (lane == 0) long_row[wid] = is_long ? row : V;
+  __syncthreads();
   const int x = threadIdx.x % kLongCols, y = threadIdx.x / kLongCols;
-  const unsigned n = *list_n;
-  for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
-    const LongRun run = list[i];
-    // the chunks it goes on into
-    unsigned last = run.chunk;
+  for (int w = 0; w < 32; ++w) {  // at most one: a long run leaves the CTA's chunks
+    if (long_row[w] >= V) continue;
+    const unsigned from = blockIdx.x * 32 + w, r = long_row[w];
+    unsigned last = from;
     for (;;) {
       const unsigned e = last + 1 + threadIdx.x;
-      const int more = __syncthreads_count(e < chunks && pair[(long long)e * L].x == run.row);
+      const int more = __syncthreads_count(e < chunks && pair[(long long)e * L].x == r);
       last += more;
-      if (more < kLongThreads) break;
+      if (more < kJoinThreads) break;
     }
     for (int c0 = blockIdx.y * kLongCols; c0 < D; c0 += gridDim.y * kLongCols) {
       const int c = c0 + x;
       float acc = 0.f;
       if (c < D) {
-        if (y == 0) acc = part[((long long)run.chunk * 2 + 1) * D + c];
+        if (y == 0) acc = part[((long long)from * 2 + 1) * D + c];
 #pragma unroll 8
-        for (unsigned e = run.chunk + 1 + y; e <= last; e += kLongRows) acc += part[(long long)e * 2 * D + c];
+        for (unsigned e = from + 1 + y; e <= last; e += kLongRows) acc += part[(long long)e * 2 * D + c];
       }
       sm[y][x] = acc;
       __syncthreads();
       if (y == 0 && c < D) {
 #pragma unroll 8
-        for (int w = 1; w < kLongRows; ++w) acc += sm[w][x];
-        grad[(long long)run.row * D + c] = from_f32<T>(acc * scale);
+        for (int k = 1; k < kLongRows; ++k) acc += sm[k][x];
+        grad[(long long)r * D + c] = from_f32<T>(acc * scale);
       }
       __syncthreads();
     }
@@ -420,7 +425,6 @@ struct EmbedWs {
   uint2* pair[2];
   unsigned *counts, *totals;
   float* part;
-  LongRun* list;
   size_t bytes;
 };
 
@@ -431,9 +435,8 @@ EmbedWs carve(void* ws, long long N, long long V, long long D) {
   EmbedWs w;
   for (int i = 0; i < 2; ++i) w.pair[i] = c.take<uint2>(s.passes > i ? N : 0);
   w.counts = c.take<unsigned>(((long long)s.tiles) << s.bits);
-  w.totals = c.take<unsigned>((1LL << s.bits) + 1);  // and the length of the list of long runs
+  w.totals = c.take<unsigned>(1LL << s.bits);
   w.part = c.take<float>((N + L - 1) / L * 2 * D);
-  w.list = c.take<LongRun>((N + L - 1) / L / kJoin + 1);
   w.bytes = c.bytes_needed();
   return w;
 }
@@ -469,20 +472,21 @@ int embedding_fwd(int dtype, const void* W, long long ldw, long long V, long lon
 int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx, long long N, long long V, long long D,
                   double scale, void* grad, void* ws, cudaStream_t s) {
   if (V <= 0 || D <= 0) return ATLB_OK;
-  const size_t esize = dtype == ATLB_F32 ? 4 : 2;
-  if (cudaMemsetAsync(grad, 0, (size_t)V * D * esize, s) != cudaSuccess) return launch_status("embedding_bwd");
-  if (N <= 0) return ATLB_OK;
+  const size_t grad_bytes = (size_t)V * D * (dtype == ATLB_F32 ? 4 : 2);
+  if (N <= 0) return cudaMemsetAsync(grad, 0, grad_bytes, s) == cudaSuccess ? ATLB_OK : launch_status("embedding_bwd");
   const SortPlan p = sort_plan(N, V);
   const EmbedWs w = carve(ws, N, V, D);
   const int bins = 1 << p.bits, L = sum_chunk(N, D);
-  unsigned* list_n = w.totals + bins;
   const void* src = idx;
   for (int i = 0; i < p.passes; ++i) {
     uint2* dst = w.pair[i & 1];
     auto pass = [&](auto first, auto items) {
       constexpr bool F = decltype(first)::value;
       constexpr int I = decltype(items)::value;
-      launch(k_sort_count<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, w.counts, list_n);
+      // enough CTAs to write the zeros as well: 64 KB each, up to two per SM
+      const int zero = F ? (int)(grad_bytes / 65536 < 296 ? grad_bytes / 65536 : 296) : 0;
+      launch(k_sort_count<F, I>, p.tiles > zero ? p.tiles : zero, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins,
+             p.tiles, w.counts, (char*)grad, (long long)grad_bytes);
       launch(k_sort_scan, (bins + 31) / 32, 1024, 0, s, w.counts, bins, p.tiles, w.totals);
       launch(k_sort_place<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, w.counts, w.totals,
              dst);
@@ -515,13 +519,11 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
       go(std::integral_constant<int, E>());
     else
       go(std::integral_constant<int, 1>());
+    // where runs are long on average, CTAs share the columns (4M events, 33 rows of 96: 90 us with one CTA to a run)
+    const unsigned share = N / V >= 16LL * L ? (unsigned)(D < 128 ? (D + kLongCols - 1) / kLongCols : 8) : 1;
     if (chunks > 1)
-      launch(k_embed_join<T>, dim3((unsigned)((chunks + 7) / 8)), kThreads, 0, s, pair, (int)N, (unsigned)V, (int)D, L,
-             (unsigned)chunks, (float)scale, w.part, (T*)grad, list_n, w.list);
-    if (chunks > kJoin)
-      launch(k_embed_join_long<T>, dim3((unsigned)(chunks / kJoin < 148 ? chunks / kJoin : 148),
-                                        (unsigned)(D < 256 ? (D + kLongCols - 1) / kLongCols : 16)),
-             kLongThreads, 0, s, pair, (int)D, L, (unsigned)chunks, (float)scale, w.part, (T*)grad, list_n, w.list);
+      launch(k_embed_join<T>, dim3((unsigned)((chunks + 31) / 32), share), kJoinThreads, 0, s, pair, (int)N, (unsigned)V, (int)D, L,
+             (unsigned)chunks, (float)scale, w.part, (T*)grad);
     return launch_status("embedding_bwd");
   });
 }

@@ -23,14 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kGroup = 32;          // rows of a group
 constexpr int kPart = 8;                      // rows between the states that the forward pass keeps for the backward pass
-#ifndef RB_M
-#define RB_M 5
-#define RB_F 5
-#define RB_B 3
-#define RB_BYTES 8
-#define RB_AHEAD 4
-#endif
-constexpr int kBytes = RB_BYTES;           // of a row per thread, where the rows are whole multiples of it
+constexpr int kBytes = 8;           // of a row per thread, where the rows are whole multiples of it
 constexpr int kSeg = 16;            // groups joined by one thread
 constexpr int kChainCols = 8, kChainSegs = 128;
 
@@ -151,10 +144,10 @@ struct Src {
 // Threads `lanes` wide on a row, E neighbouring columns each; the CTA's groups are one chunk.  BWD walks from the last
 // row to the first: in = dL/dh, and the state is u.  prefix: the map from the chunk's entry to the group's; chunk: the
 // whole chunk's map.
-constexpr int kAhead = RB_AHEAD;  // rows in flight per thread
+constexpr int kAhead = 4;  // rows in flight per thread
 
 template <typename T, int E, int KIND, bool BWD>
-__global__ void __launch_bounds__(kThreads, RB_M) k_rec_map(RecShape S, Src<T> gate, Src<T> in, const float* __restrict__ s0,
+__global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate, Src<T> in, const float* __restrict__ s0,
                                                       uint2* __restrict__ prefix, uint2* __restrict__ chunk) {
   __shared__ uint2 sm[kThreads * E];
   __shared__ uint2 seg[32 * E];  // segments x columns: 16 E, or 32 E where a warp takes a row
@@ -314,7 +307,7 @@ __device__ __forceinline__ void group_state(const RecShape& S, const uint2* pref
 
 // ------------------------------------------------------------------------------------------------ replay, forward
 template <typename T, int E, int KIND>
-__global__ void __launch_bounds__(kThreads, RB_F) k_rec_fwd(RecShape S, Src<T> gate, Src<T> x, const float* __restrict__ h0,
+__global__ void __launch_bounds__(kThreads, 5) k_rec_fwd(RecShape S, Src<T> gate, Src<T> x, const float* __restrict__ h0,
                                                       const uint2* __restrict__ prefix,
                                                       const float* __restrict__ state, T* __restrict__ h,
                                                       float* __restrict__ hT, float* __restrict__ saved) {
@@ -376,11 +369,35 @@ __global__ void __launch_bounds__(kThreads, RB_F) k_rec_fwd(RecShape S, Src<T> g
     rows(std::true_type());
 }
 
+// One row per window (a step of running windows): row by row in parallel, E columns per thread.
+template <typename T, int E, int KIND>
+__global__ void __launch_bounds__(kThreads) k_rec_step(RecShape S, Src<T> gate, Src<T> x, const float* __restrict__ h0,
+                                                       T* __restrict__ h, float* __restrict__ hT,
+                                                       float* __restrict__ saved) {
+  const int per_row = S.D / E;
+  const long long i = blockIdx.x * (long long)kThreads + threadIdx.x, n = i / per_row;
+  const int c = (int)(i - n * per_row) * E;
+  if (n >= S.N) return;
+  const Pack<T, E> gp = load_pack<T, E>(gate.p + n * gate.ld + c), xp = load_pack<T, E>(x.p + n * x.ld + c);
+  Pack<T, E> o;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    float a, w, v;
+    row_terms<KIND>(to_f32(gp.v[e]), to_f32(xp.v[e]), &a, &w, &v);
+    const float s = fmaf(a, h0 ? h0[n * S.D + c + e] : 0.f, v);
+    o.v[e] = from_f32<T>(s);
+    if (hT) hT[n * S.D + c + e] = s;
+    // every row begins a window, so the backward pass takes h0 in the place of what it finds here
+    if (saved && n % kPart == 0) saved[n / kPart * S.D + c + e] = 0.f;
+  }
+  store_pack(h + n * S.D + c, o);
+}
+
 // ------------------------------------------------------------------------------------------------ replay, backward
 // lanes_b threads on a row, E columns each (4 bytes), a group per `lanes_b` threads.  Each part of the group, the last
 // one first: its rows in registers, the states forward from the one the forward pass kept, then u backward.
 template <typename T, int E, int KIND>
-__global__ void __launch_bounds__(kThreads, RB_B) k_rec_bwd(RecShape S, int lanes_b, Src<T> gate, Src<T> x, Src<T> gh,
+__global__ void __launch_bounds__(kThreads, 3) k_rec_bwd(RecShape S, int lanes_b, Src<T> gate, Src<T> x, Src<T> gh,
                                                          const float* __restrict__ h0, const float* __restrict__ ghT,
                                                          const float* __restrict__ saved,
                                                          const uint2* __restrict__ prefix,
@@ -485,9 +502,9 @@ RecWs carve(void* ws, long long N, long long D) {
   return w;
 }
 
-// The state before each window's rows, for windows that have none: copied ahead of the kernels, which overwrite it.
-int fill_state(float* dst, const float* src, long long n, cudaStream_t s) {
-  if (!dst || n <= 0) return ATLB_OK;
+// Packed windows may be empty: what theirs are to hold is copied ahead of the kernels, which overwrite the others'.
+int fill_state(float* dst, const float* src, long long n, bool packed, cudaStream_t s) {
+  if (!dst || n <= 0 || !packed) return ATLB_OK;
   const cudaError_t e = src ? cudaMemcpyAsync(dst, src, n * sizeof(float), cudaMemcpyDeviceToDevice, s)
                             : cudaMemsetAsync(dst, 0, n * sizeof(float), s);
   return e == cudaSuccess ? ATLB_OK : launch_status("recurrence");
@@ -552,7 +569,7 @@ int recurrence_fwd(int dtype, int kind, const void* gate, long long ldg, const v
                    const long long* b, long long N, long long B, long long D, const float* h0, void* h, float* hT,
                    float* saved, void* ws, cudaStream_t s) {
   if (D <= 0) return ATLB_OK;
-  if (int st = fill_state(hT, h0, B * D, s)) return st;
+  if (int st = fill_state(hT, h0, B * D, b || N <= 0, s)) return st;
   if (N <= 0) return ATLB_OK;
   const RecWs w = carve(ws, N, D);
   return with_dtype(dtype, [&](auto tag) {
@@ -568,6 +585,11 @@ int recurrence_fwd(int dtype, int kind, const void* gate, long long ldg, const v
         constexpr int E = decltype(el)::value;
         const RecShape S = make_shape(N, B, D, b, E);
         const int W = S.lanes * E;
+        if (!b && S.T == 1) {
+          launch(k_rec_step<T, E, KIND>, (unsigned)((N * (D / E) + kThreads - 1) / kThreads), kThreads, 0, s, S, sg, sx, h0,
+                 (T*)h, hT, saved);
+          return launch_status("recurrence_fwd");
+        }
         find_states<T, E, KIND, false>(S, sg, sx, h0, w, s);
         launch(k_rec_fwd<T, E, KIND>, dim3(S.chunks, (S.D + W - 1) / W), kThreads, 0, s, S, sg, sx, h0, w.prefix, w.state,
                (T*)h, hT, saved);
@@ -584,7 +606,7 @@ int recurrence_bwd(int dtype, int kind, const void* gate, long long ldg, const v
                    const void* gh, long long ldgh, const float* ghT, void* ggate, void* gx, float* gh0, void* ws,
                    cudaStream_t s) {
   if (D <= 0) return ATLB_OK;
-  if (int st = fill_state(gh0, ghT, B * D, s)) return st;
+  if (int st = fill_state(gh0, ghT, B * D, b || N <= 0, s)) return st;
   if (N <= 0) return ATLB_OK;
   const RecWs w = carve(ws, N, D);
   return with_dtype(dtype, [&](auto tag) {

@@ -397,11 +397,12 @@ int atlb_rng_normal2(uint64_t seed, uint64_t call, int64_t n, float* out, atlb_s
  * features per event) and whose output the objectives score.  No counterpart in the reference's ops.
  * Element types (dtype): ATLB_F32, ATLB_BF16, ATLB_F16; all arrays of one call marked `void*` have that type.  Rows
  * are contiguous; the row stride ld* (in elements, >= 0) of an input may differ from D, outputs have stride D.
- * Sums, states and products are fp32, and every output is rounded once.  D <= ATLB_SEQ_MAX_D; N and row strides below
- * 2^31.
+ * Sums, states and products are fp32, and every output is rounded once.  N <= ATLB_SEQ_MAX_N, D <= ATLB_SEQ_MAX_D, row
+ * strides below 2^31 in the row lookup; N * D may exceed 32 bits.
  * ---------------------------------------------------------------------------------------------- */
 enum { ATLB_F32 = 0, ATLB_BF16 = 1, ATLB_F16 = 2 };
 #define ATLB_SEQ_MAX_D (1 << 20)
+#define ATLB_SEQ_MAX_N ((1LL << 31) - 65536) /* rows are counted in 32 bits, with room behind the last */
 
 /* Row lookup: out[n, :] = scale * weight[idx[n], :], zero where idx[n] lies outside [0, V) (as the gather reads zero
  * outside the image).  weight (V, D) with row stride ldw, idx (N), out (N, D). */

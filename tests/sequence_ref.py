@@ -56,10 +56,11 @@ def embedding(weight, idx, scale, g=None):
 
 
 # ------------------------------------------------------------------------------------------------ dropout
-def philox_words(n, seed, call):
-    """Words 0 .. n-1 of the dropout stream: four per counter (i // 4, 2^31 + (i // 4 >> 32), call)."""
+def philox_words(n, seed, call, start=0):
+    """Words start .. start + n - 1 of the dropout stream (start a multiple of 4): four per counter
+    (i // 4, 2^31 + (i // 4 >> 32), call)."""
     u64, m = np.uint64, np.uint64(0xFFFFFFFF)
-    q = np.arange((n + 3) // 4, dtype=np.uint64)
+    q = np.arange((n + 3) // 4, dtype=np.uint64) + u64(start // 4)
     c = [q & m, (q >> u64(32)) | u64(1 << 31), np.full_like(q, call & 0xFFFFFFFF), np.full_like(q, call >> 32)]
     k = [seed & 0xFFFFFFFF, seed >> 32]
     for _ in range(10):

@@ -392,6 +392,79 @@ def test_operators_on_another_stream_and_in_graphs():
         assert all(same_bits(p, q) for p, q in zip(ref, o))
 
 
+def test_operators_from_two_threads():
+    """Calls from two threads, each on its own stream, give the bits of calls one after the other."""
+    import threading
+    args = []
+    for k in range(2):
+        w, idx, g = lookup_inputs(20000, 900, 64, torch.float32, 40 + k, "skew")
+        args.append((w.requires_grad_(), idx, g, gates("sigmoid", 20000, 64, torch.float32, 50 + k)))
+
+    def step(w, idx, g, gate):
+        h = x_b200.linear_recurrence(gate, x_b200.dropout(x_b200.embedding(w, idx), 0.3, 1, 2), B=4)
+        return h.detach(), torch.autograd.grad(h, [w], g)[0]
+
+    ref, out = [step(*a) for a in args], [[], []]
+    torch.cuda.synchronize()
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                out[k].append(step(*args[k]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(out[k]) == 5
+        for o in out[k]:
+            assert all(same_bits(p, q) for p, q in zip(ref[k], o))
+
+
+# ------------------------------------------------------------------------------------------------ offsets past 32 bits
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows, whose offsets do not fit 32 bits, against the float64 statements."""
+    N, D, dtype = 35_000_000, 64, torch.bfloat16
+    assert N * D > 2**31
+    # dropout: elements near the end
+    x = torch.zeros(N, D, dtype=dtype, device=DEV)
+    tail = slice(N - 16, N)
+    x[tail] = randn(16, D, seed=1, dtype=dtype)
+    y = x_b200.dropout(x, 0.4, 9, 3)
+    keep = (R.philox_words(16 * D, 9, 3, start=(N - 16) * D) >= np.uint64(np.floor(0.4 * 2.0**32 + 0.5))).reshape(16, D)
+    ref = np.where(keep, R.f64(x[tail]) / 0.6, 0.0)
+    R.check(y[tail], ref, 2 * R.U * np.abs(ref))
+    del y
+    # recurrence: a short last window behind one long one
+    b = torch.zeros(N, dtype=torch.long, device=DEV)
+    b[tail] = 1
+    gate = torch.zeros(N, D, dtype=dtype, device=DEV)
+    gate[tail] = gates("sigmoid", 16, D, dtype, 2)
+    gate.requires_grad_(), x.requires_grad_()
+    h, st = x_b200.linear_recurrence(gate, x, b=b, B=2, return_state=True)
+    g_state = randn(2, D, seed=3)
+    gg, gx = torch.autograd.grad(st, [gate, x], g_state)
+    r = R.recurrence("sigmoid", R.f64(gate[tail]), R.f64(x[tail]), np.zeros(16, int), 1, None, np.zeros((16, D)),
+                     R.f64(g_state[1:]))
+    R.check(h[tail], *r["h"])
+    R.check(st[1:], *r["state"])
+    R.check(gg[tail], *r["dgate"])
+    R.check(gx[tail], *r["dx"])
+    del h, st, gate, gg, gx, b
+    # lookup: the output's last rows, and their gradients (x as the incoming one)
+    w = randn(3, D, seed=4, dtype=dtype).requires_grad_()
+    idx = torch.full((N,), -1, device=DEV)
+    idx[tail] = torch.arange(16, device=DEV) % 3
+    out = x_b200.embedding(w, idx, 0.5)
+    (gw,) = torch.autograd.grad(out, [w], x.detach())
+    fwd, bwd = R.embedding(R.f64(w), idx[tail].cpu().numpy(), 0.5, R.f64(x[tail]))
+    R.check(out[tail], *fwd)
+    R.check(gw, *bwd)
+
+
 # ------------------------------------------------------------------------------------------------ together
 def test_event_sequence_model_under_the_objective():
     """Events looked up by pixel, dropped out, run through the recurrence; its end states give each window's motion,

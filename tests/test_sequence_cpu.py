@@ -31,6 +31,8 @@ def test_cpu_tensors_are_refused():
     ("atlb_embedding_fwd", (0, P, -1, 4, 4, P, 2, 1.0, P, None), _lib.ATLB_ERR_ARG, b"negative"),
     ("atlb_embedding_fwd", (0, P, 4, 2**31, 4, P, 2, 1.0, P, None), _lib.ATLB_ERR_OVERFLOW, b"rows"),
     ("atlb_embedding_fwd", (0, P, 4, 4, 2**21, P, 2, 1.0, P, None), _lib.ATLB_ERR_OVERFLOW, b"columns"),
+    ("atlb_embedding_fwd", (0, P, 2**31, 4, 4, P, 2, 1.0, P, None), _lib.ATLB_ERR_OVERFLOW, b"stride"),
+    ("atlb_embedding_bwd", (0, P, 4, P, 2**31 - 1, 4, 4, 1.0, P, P, 16, None), _lib.ATLB_ERR_OVERFLOW, b"rows"),
     ("atlb_embedding_bwd", (0, P, 4, P, 2, 4, 4, 1.0, P, P, 16, None), _lib.ATLB_ERR_WORKSPACE, b"workspace"),
     ("atlb_embedding_bwd", (0, P, 4, P, 2**31, 4, 4, 1.0, P, P, 16, None), _lib.ATLB_ERR_OVERFLOW, b"rows"),
     ("atlb_dropout", (0, P, None, 4, 1.5, 0, 0, None, P, None), _lib.ATLB_ERR_ARG, b"p ="),

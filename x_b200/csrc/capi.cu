@@ -642,7 +642,7 @@ static int check_seq(int dtype, int64_t N, int64_t D, const char* fn) {
     set_error("%s: unknown dtype %d", fn, dtype);
     return ATLB_ERR_ARG;
   }
-  if (N > (1LL << 31) - 1 || D > ATLB_SEQ_MAX_D) {
+  if (N > ATLB_SEQ_MAX_N || D > ATLB_SEQ_MAX_D) {
     set_error("%s: %lld rows of %lld columns exceed the kernels' sizes", fn, (long long)N, (long long)D);
     return ATLB_ERR_OVERFLOW;
   }

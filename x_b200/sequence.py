@@ -78,8 +78,8 @@ def _embedding_fwd(weight, idx, scale):
     dev = w.device
     with _on(dev):
         out = torch.empty(*idx.shape, D, dtype=w.dtype, device=dev)
-        L.check(L.load_library().atlb_embedding_fwd(L.DTYPES[w.dtype], w.data_ptr(), ldw, V, D, idx.data_ptr(), idx.numel(),
-                                           scale, out.data_ptr(), _stream(dev)), "embedding")
+        L.check(L.load_library().atlb_embedding_fwd(L.DTYPES[w.dtype], w.data_ptr(), ldw, V, D, idx.data_ptr(),
+                                                    idx.numel(), scale, out.data_ptr(), _stream(dev)), "embedding")
     return out
 
 
@@ -132,8 +132,8 @@ def _dropout_run(x, residual, p, seed, call):
     with _on(dev):
         out = torch.empty_like(x)
         L.check(L.load_library().atlb_dropout(L.DTYPES[x.dtype], x.data_ptr(), _addr(residual), x.numel(), p, seed,
-                                     0 if dev_call is not None else call, _addr(dev_call), out.data_ptr(),
-                                     _stream(dev)), "dropout")
+                                              0 if dev_call is not None else call, _addr(dev_call), out.data_ptr(),
+                                              _stream(dev)), "dropout")
     return out
 
 
@@ -162,8 +162,9 @@ def dropout(x: torch.Tensor, p: float, seed: int, call=0, residual: torch.Tensor
     The mask is a function of (seed, call) and the element's index and is never stored: the backward pass draws it
     again.  Give every place and step that drops its own (seed, call), for instance
     ``dropout(x, p, draws.seed, draws.next_call())`` with a :class:`x_b200.rng.DeviceDraws`; the same pair gives the
-    same mask.  ``call`` may be a one-element int64 tensor on x's device instead, read when the kernel runs: a captured
-    CUDA graph that adds to it after its backward pass drops anew on every replay."""
+    same mask, and so does every replay of a CUDA graph that captured an integer ``call``.  ``call`` may be a one-element
+    int64 tensor on x's device instead, read when the kernel runs: a captured graph that adds to it after its backward
+    pass drops anew on every replay."""
     dev = _need("dropout", x=x, residual=residual)
     _need_dtype("dropout", "x", x, L.DTYPES)
     if not 0.0 <= p <= 1.0:

@@ -16,10 +16,10 @@ constexpr int kThreads = 256;
 // ------------------------------------------------------------------------------------------------ forward
 // A group of `lanes` threads (up to 32) takes kRowsEach rows, E neighbouring columns per thread: the rows' numbers, then
 // all their loads, then the stores.  Groups need not divide a warp: rows of 96 fp16 columns take 12 threads.
-constexpr int kRowsEach = 4;
+constexpr int kRowsEach = 3;  // four at 5 CTAs per SM 45 instead of 40 us for 1M rows of 64 bf16 columns, eight 80
 
 template <typename T, int E>
-__global__ void __launch_bounds__(kThreads, 5) k_embed_fwd(const T* __restrict__ W, int ldw, int V, int D,
+__global__ void __launch_bounds__(kThreads, 6) k_embed_fwd(const T* __restrict__ W, int ldw, int V, int D,
                                                            const long long* __restrict__ idx, int N, float scale,
                                                            int lanes, T* __restrict__ out) {
   const int per = kThreads / lanes, mine = threadIdx.x / lanes, c = (blockIdx.y * lanes + threadIdx.x % lanes) * E;
@@ -131,33 +131,43 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* sm, unsigne
   return before + inc - v;
 }
 
-// A CTA per 32 digits: their counts over the tiles become offsets within the digit.  A thread sums a run of tiles, the
-// 32 runs of a digit are joined, and the thread walks its run again.
-__global__ void __launch_bounds__(1024) k_sort_scan(unsigned* __restrict__ counts, int bins, int tiles,
-                                                    unsigned* __restrict__ totals) {
-  __shared__ unsigned sm[32][33];
-  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, d = blockIdx.x * 32 + x;
-  const int run = (tiles + 31) / 32, t0 = y * run, t1 = min(t0 + run, tiles);
+// A CTA per 8 digits: their counts over the tiles become offsets within the digit.  A thread sums a run of tiles, the
+// 128 runs of a digit are joined, and the thread walks its run again.
+constexpr int kScanDigits = 8, kScanRuns = 128;
+__global__ void __launch_bounds__(kScanDigits * kScanRuns) k_sort_scan(unsigned* __restrict__ counts, int bins, int tiles,
+                                                                       unsigned* __restrict__ totals) {
+  __shared__ unsigned sm[kScanDigits][kScanRuns + 1];
+  const int x = threadIdx.x % kScanDigits, y = threadIdx.x / kScanDigits, d = blockIdx.x * kScanDigits + x;
+  const int run = (tiles + kScanRuns - 1) / kScanRuns, t0 = y * run, t1 = min(t0 + run, tiles);
   unsigned sum = 0;
   if (d < bins) {
 #pragma unroll 8
     for (int t = t0; t < t1; ++t) sum += counts[(long long)t * bins + d];
   }
-  sm[y][x] = sum;
+  sm[x][y] = sum;
   __syncthreads();
-  // the warp of digit row y joins the 32 runs of digit y
-  unsigned inc = sm[x][y];
-  const unsigned own = inc;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  if (wid < kScanDigits) {  // a warp per digit, four runs a lane
+    unsigned v[4], inc = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned u = __shfl_up_sync(0xffffffffu, inc, o);
-    if (x >= o) inc += u;
+    for (int k = 0; k < 4; ++k) inc += v[k] = sm[wid][lane * 4 + k];
+    const unsigned own = inc;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    unsigned at = inc - own;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      sm[wid][lane * 4 + k] = at;
+      at += v[k];
+    }
+    if (lane == 31 && blockIdx.x * kScanDigits + wid < bins) totals[blockIdx.x * kScanDigits + wid] = inc;
   }
-  sm[x][y] = inc - own;
-  if (x == 31 && blockIdx.x * 32 + y < bins) totals[blockIdx.x * 32 + y] = inc;
   __syncthreads();
   if (d >= bins) return;
-  unsigned at = sm[y][x];
+  unsigned at = sm[x][y];
 #pragma unroll 8
   for (int t = t0; t < t1; ++t) {
     const unsigned c = counts[(long long)t * bins + d];
@@ -274,10 +284,10 @@ SortPlan sort_plan(long long N, long long V) {
 // A group of `lanes` threads walks the L sorted pairs of one chunk, keeping E columns per thread in fp32, and
 // writes a gradient row when its run ends inside the chunk.  A run that came in from the chunk before leaves its
 // sum in part[chunk][0], one that goes on into the next chunk in part[chunk][1] (in [0] if it does both).
-constexpr int kAhead = 4;  // rows in flight per thread
+constexpr int kAhead = 4;  // rows in flight per thread; the registers for it are worth more than a fourth CTA (47 -> 37 us)
 
 template <typename T, int E>
-__global__ void __launch_bounds__(kThreads, 4) k_embed_sum(const T* __restrict__ g, int ldg,
+__global__ void __launch_bounds__(kThreads, 3) k_embed_sum(const T* __restrict__ g, int ldg,
                                                            const uint2* __restrict__ pair, int N, unsigned V, int D,
                                                            int L, int lanes, float scale, T* __restrict__ grad,
                                                            float* __restrict__ part) {
@@ -414,10 +424,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_embed_join(const uint2* __rest
 // Threads on a row of D columns, E each.
 int group_lanes(long long D, int E) { return D >= 32LL * E ? 32 : D < 1 ? 1 : (int)((D + E - 1) / E); }
 
-// Pairs per chunk: one wave of groups on the GPU (148 SMs of 4 CTAs, groups of 16-byte threads on 16-bit rows), so that
+// Pairs per chunk: one wave of groups on the GPU (148 SMs of 3 CTAs, groups of 16-byte threads on 16-bit rows), so that
 // all end together.
 int sum_chunk(long long N, long long D) {
-  const long long wave = 148LL * 4 * (kThreads / group_lanes(D, 8)), L = (N + wave - 1) / wave;
+  const long long wave = 148LL * 3 * (kThreads / group_lanes(D, 8)), L = (N + wave - 1) / wave;
   return (int)(L < 16 ? 16 : L);
 }
 
@@ -487,7 +497,7 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
       const int zero = F ? (int)(grad_bytes / 65536 < 296 ? grad_bytes / 65536 : 296) : 0;
       launch(k_sort_count<F, I>, p.tiles > zero ? p.tiles : zero, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins,
              p.tiles, w.counts, (char*)grad, (long long)grad_bytes);
-      launch(k_sort_scan, (bins + 31) / 32, 1024, 0, s, w.counts, bins, p.tiles, w.totals);
+      launch(k_sort_scan, (bins + kScanDigits - 1) / kScanDigits, kScanDigits * kScanRuns, 0, s, w.counts, bins, p.tiles, w.totals);
       launch(k_sort_place<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, w.counts, w.totals,
              dst);
     };

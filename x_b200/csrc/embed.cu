@@ -131,6 +131,9 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* sm, unsigne
   return before + inc - v;
 }
 
+// Up to this many tiles, each CTA of the placement sums the counts before its own itself: a launch less per pass.
+constexpr int kFewTiles = 64;
+
 // A CTA per 8 digits: their counts over the tiles become offsets within the digit.  A thread sums a run of tiles, the
 // 128 runs of a digit are joined, and the thread walks its run again.
 constexpr int kScanDigits = 8, kScanRuns = 128;
@@ -181,7 +184,8 @@ __global__ void __launch_bounds__(kScanDigits * kScanRuns) k_sort_scan(unsigned*
 // side by side: scattered one by one, 1M pairs take 19 us a pass.
 template <bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restrict__ src, long long N, unsigned V,
-                                                             int shift, int bins, const unsigned* __restrict__ counts,
+                                                             int shift, int bins, int tiles,
+                                                             const unsigned* __restrict__ counts,
                                                              const unsigned* __restrict__ totals,
                                                              uint2* __restrict__ out) {
   constexpr int kTile = kSortThreads * ITEMS;
@@ -199,9 +203,22 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restr
   unsigned carry = 0;
   for (int d0 = 0; d0 < bins; d0 += kSortThreads) {
     const int d = d0 + threadIdx.x;
-    unsigned total;
-    const unsigned ex = block_scan<kSortThreads>(d < bins ? totals[d] : 0, sm, &total);
-    if (d < bins) start[d] = carry + ex + counts[(long long)blockIdx.x * bins + d];
+    unsigned all = 0, before = 0, total;  // pairs of the digit, in all tiles and in those before this one
+    if (d < bins) {
+      if (tiles > kFewTiles) {
+        all = totals[d];
+        before = counts[(long long)blockIdx.x * bins + d];
+      } else {
+#pragma unroll 8
+        for (int t = 0; t < tiles; ++t) {
+          const unsigned c = counts[(long long)t * bins + d];
+          all += c;
+          before += t < blockIdx.x ? c : 0;
+        }
+      }
+    }
+    const unsigned ex = block_scan<kSortThreads>(all, sm, &total);
+    if (d < bins) start[d] = carry + ex + before;
     carry += total;
   }
   unsigned at[ITEMS];  // lanes of the same digit, then the rank among the warp's pairs of it, then the place in the tile
@@ -497,9 +514,10 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
       const int zero = F ? (int)(grad_bytes / 65536 < 296 ? grad_bytes / 65536 : 296) : 0;
       launch(k_sort_count<F, I>, p.tiles > zero ? p.tiles : zero, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins,
              p.tiles, w.counts, (char*)grad, (long long)grad_bytes);
-      launch(k_sort_scan, (bins + kScanDigits - 1) / kScanDigits, kScanDigits * kScanRuns, 0, s, w.counts, bins, p.tiles, w.totals);
-      launch(k_sort_place<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, w.counts, w.totals,
-             dst);
+      if (p.tiles > kFewTiles)
+        launch(k_sort_scan, (bins + kScanDigits - 1) / kScanDigits, kScanDigits * kScanRuns, 0, s, w.counts, bins, p.tiles, w.totals);
+      launch(k_sort_place<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, p.tiles,
+             w.counts, w.totals, dst);
     };
     auto sized = [&](auto first) {
       if (p.large)

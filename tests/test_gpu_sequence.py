@@ -324,6 +324,24 @@ def test_recurrence_values():
     assert same_bits(torch.autograd.grad(st, [h0], x[:3])[0], x[:3])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_recurrence_saturated_gates(dtype):
+    """A gate of +inf (or far above) keeps the state, one of -inf (or far below) takes x, both to the bit; no NaN in the
+    gradients."""
+    N, D = 70, 8
+    big = 200.0 if dtype == torch.float16 else 1e4
+    gate = torch.empty(N, D, dtype=dtype, device=DEV)
+    gate[0], gate[1:40], gate[40:] = -big, big, -float("inf")
+    gate[5], gate[41] = float("inf"), -big
+    gate.requires_grad_()
+    x = randn(N, D, seed=1, dtype=dtype).requires_grad_()
+    h = x_b200.linear_recurrence(gate, x)
+    assert torch.equal(h[:40], x[:1].expand(40, D)) and torch.equal(h[40:], x[40:])
+    gg, gx = torch.autograd.grad(h.float().sum(), [gate, x])
+    assert torch.isfinite(gg).all() and torch.isfinite(gx).all()
+    assert torch.equal(gx[40:], torch.ones_like(gx[40:])) and (gx[1:40] == 0).all()
+
+
 @pytest.mark.parametrize("kind", ["sigmoid", "decay"])
 def test_recurrence_step_by_step(kind):
     """A window read whole, in two parts and row by row, the state handed on, gives the same states up to rounding."""

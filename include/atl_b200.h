@@ -397,7 +397,7 @@ int atlb_rng_normal2(uint64_t seed, uint64_t call, int64_t n, float* out, atlb_s
  * features per event) and whose output the objectives score.  No counterpart in the reference's ops.
  * Element types (dtype): ATLB_F32, ATLB_BF16, ATLB_F16; all arrays of one call marked `void*` have that type.  Rows
  * are contiguous; the row stride ld* (in elements, >= 0) of an input may differ from D, outputs have stride D.
- * Sums, states and products are fp32, and every output is rounded once.  N <= ATLB_SEQ_MAX_N, D <= ATLB_SEQ_MAX_D, row
+ * Outputs must not overlap inputs.  Sums, states and products are fp32, and every output is rounded once.  N <= ATLB_SEQ_MAX_N, D <= ATLB_SEQ_MAX_D, row
  * strides below 2^31 in the row lookup; N * D may exceed 32 bits.
  * ---------------------------------------------------------------------------------------------- */
 enum { ATLB_F32 = 0, ATLB_BF16 = 1, ATLB_F16 = 2 };
@@ -427,8 +427,9 @@ int atlb_dropout(int dtype, const void* x, const void* residual, int64_t n, doub
 /* Gated linear recurrence over the rows of packed windows, per column:
  *   ATLB_REC_DECAY    h_t = gate_t h_(t-1) + x_t
  *   ATLB_REC_SIGMOID  h_t = a_t h_(t-1) + (1 - a_t) x_t,  a_t = 1 / (1 + exp(-gate_t))
- * gate, x (N, D); b (N) the window of each row, the rows of a window contiguous (events sorted by (b, t) are); rows
- * with b outside [0, B) get h = 0 and no gradient.  b NULL: B equal windows of N / B rows (N a multiple of B).
+ * gate, x (N, D); b (N) the window of each row, the rows of a window contiguous (events sorted by (b, t) are; otherwise
+ * each run of equal b starts from h0, and which run's hT and gh0 remain is open); rows with b outside [0, B) get h = 0
+ * and no gradient.  b NULL: B equal windows of N / B rows (N a multiple of B).
  * h0 (B, D) fp32: the state before each window's first row, NULL for zero.  h (N, D); hT (B, D) fp32 or NULL: the
  * state after each window's last row (h0 for a window without rows).  saved: NULL, or
  * atlb_recurrence_saved_bytes(N, D) bytes that the backward pass takes. */

@@ -17,7 +17,7 @@ constexpr int kThreads = 256;
 // A group of `lanes` threads (up to 32) takes kRowsEach rows, E neighbouring columns per thread: the rows' numbers, then
 // all their loads, then the stores.  Groups need not divide a warp: rows of 96 fp16 columns take 12 threads.  1M rows of
 // 64 bf16 columns from 307200: 42 us (175 MB, 4.2 TB/s); 4M of 96 fp16 columns from 33 rows: 172 us (800 MB, 4.7 TB/s).
-constexpr int kRowsEach = 3;  // four at 5 CTAs per SM 45 instead of 40 us for 1M rows of 64 bf16 columns, eight 80
+constexpr int kRowsEach = 3;  // four (5 CTAs per SM) take 45 us where three take 42, eight (4 CTAs) 80
 
 template <typename T, int E>
 __global__ void __launch_bounds__(kThreads, 6) k_embed_fwd(const T* __restrict__ W, int ldw, int V, int D,
@@ -55,9 +55,10 @@ __global__ void __launch_bounds__(kThreads, 6) k_embed_fwd(const T* __restrict__
 
 // ------------------------------------------------------------------------------------------------ sort
 // Least-significant-digit radix sort of (row, event) pairs, up to kMaxBits per pass.  A tile is 512 * ITEMS
-// neighbouring pairs; every pass counts the tiles' digits, scans the counts and places the pairs.  Tiles
-// of 4096 pairs spread the work per digit (a place per warp and digit to clear and to sum) over more pairs; below 64 tiles
-// of that size the GPU would idle, and tiles of 2048 are taken.
+// neighbouring pairs; every pass counts the tiles' digits, scans the counts and places the pairs.  Tiles of 4096 pairs
+// spread the work per digit (a place per warp and digit to clear and to sum) over more pairs: lookup and gradient of 1M
+// events 190 us against 195 with 2048.  Below 64 tiles of that size the GPU would idle, and tiles of 2048 are taken.
+// 1M pairs take 20 us a placement, bound by the latency of its steps (28 % of issue slots, 5 % of DRAM).
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxBits = 10;
@@ -305,7 +306,7 @@ SortPlan sort_plan(long long N, long long V) {
 // sum in part[chunk][0], one that goes on into the next chunk in part[chunk][1] (in [0] if it does both).  Bound by its
 // scattered row reads: 1M rows of 64 bf16 columns 40 us (137 MB from DRAM, 3.8 TB/s), 4M of 96 fp16 columns 171 us
 // (995 MB, 5.8 TB/s; rows of 192 bytes fetch parts of lines that others need later).
-constexpr int kAhead = 4;  // rows in flight per thread; the registers for it are worth more than a fourth CTA (47 -> 37 us)
+constexpr int kAhead = 4;  // rows in flight per thread, at 3 CTAs per SM: 4 CTAs with spilled registers took 47 us
 
 template <typename T, int E>
 __global__ void __launch_bounds__(kThreads, 3) k_embed_sum(const T* __restrict__ g, int ldg,
@@ -519,7 +520,8 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
       launch(k_sort_count<F, I>, p.tiles > zero ? p.tiles : zero, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins,
              p.tiles, w.counts, (char*)grad, (long long)grad_bytes);
       if (p.tiles > kFewTiles)
-        launch(k_sort_scan, (bins + kScanDigits - 1) / kScanDigits, kScanDigits * kScanRuns, 0, s, w.counts, bins, p.tiles, w.totals);
+        launch(k_sort_scan, (bins + kScanDigits - 1) / kScanDigits, kScanDigits * kScanRuns, 0, s, w.counts, bins,
+               p.tiles, w.totals);
       launch(k_sort_place<F, I>, p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins, p.tiles,
              w.counts, w.totals, dst);
     };
@@ -554,8 +556,8 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
     // where runs are long on average, CTAs share the columns (4M events, 33 rows of 96: 40 us, 90 with one CTA to a run)
     const unsigned share = N / V >= 16LL * L ? (unsigned)(D < 128 ? (D + kLongCols - 1) / kLongCols : 8) : 1;
     if (chunks > 1)
-      launch(k_embed_join<T>, dim3((unsigned)((chunks + 31) / 32), share), kJoinThreads, 0, s, pair, (int)N, (unsigned)V, (int)D, L,
-             (unsigned)chunks, (float)scale, w.part, (T*)grad);
+      launch(k_embed_join<T>, dim3((unsigned)((chunks + 31) / 32), share), kJoinThreads, 0, s, pair, (int)N, (unsigned)V,
+             (int)D, L, (unsigned)chunks, (float)scale, w.part, (T*)grad);
     return launch_status("embedding_bwd");
   });
 }

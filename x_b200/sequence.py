@@ -243,8 +243,9 @@ def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, b: torch.Tensor | Non
         kind="decay"    h_t = gate_t h_(t-1) + x_t          (exp(-dt / tau): decaying event traces)
 
     gate, x (N, D), one dtype; slices of a wider projection are taken as they are.  ``b`` (N,) int64 is the window of
-    each row in [0, B), the rows of a window contiguous, as in events sorted by (b, t); rows with any other value
-    (padding, -1) get h = 0 and no gradient, and what they hold reaches nothing.  Without ``b`` the rows are B equal
+    each row in [0, B), the rows of a window contiguous, as in events sorted by (b, t) (not checked: every run of equal
+    ``b`` starts from h0, and which run's state is returned is open); rows with any other value (padding, -1) get h = 0
+    and no gradient, and what they hold reaches nothing.  Without ``b`` the rows are B equal
     windows: a (B, T, D) batch is ``flatten(0, 1)``.  ``h0`` (B, D) float32 is the state before each window's first
     row (default zero).  Returns h (N, D), or (h, state) with ``return_state``: state (B, D) float32 after each
     window's last row (h0 where a window has none), to be given as the next call's ``h0``; one row per window is one

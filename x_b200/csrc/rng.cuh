@@ -5,7 +5,8 @@
 //
 // Stream layout of this library: the draw for item i (an event or an anchor) of call number c uses the
 // counter (i, stream, c mod 2^32, c / 2^32) and the key (seed mod 2^32, seed / 2^32); stream 0 gives the
-// dequantisation jitter u (two uniforms), stream 1 the anchor smoothing noise z (two normals).
+// dequantisation jitter u (two uniforms), stream 1 the anchor smoothing noise z (two normals).  The dropout of
+// dropout.cu draws from counters with bit 31 of the second word set.
 //   uniform: (w >> 8) * 2^-24, in [0, 1) with 24 random bits (the fp32 mantissa)
 //   normal : Box-Muller on the first two words, r = sqrt(-2 log u1) with u1 = ((w0 >> 8) + 1) * 2^-24 in (0, 1],
 //            angle 2 pi u2: (r cos, r sin)

@@ -13,45 +13,38 @@ run.  There is no CPU path, and the gradients are not differentiable again.
 """
 from __future__ import annotations
 
-import contextlib
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
 _MASK64 = 2**64 - 1
+_INDEX_TYPES = (torch.int64, torch.int32, torch.int16, torch.uint8)
+_current_device = torch._C._cuda_getDevice
+# the device's current stream as an integer: a Stream object costs several microseconds to make
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 # ------------------------------------------------------------------------------------------- arguments
-def _need(what: str, **tensors):
-    """Every given tensor on one CUDA device; the first decides."""
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"x_b200.{what}: {name} must be a CUDA tensor (there is no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"x_b200.{what}: {name} lies on {t.device}, the other tensors on {dev}")
-    return dev
+# A small call is bound by the host, so the checks are made on integers, and what they refuse is put into words here.
+def _device(what: str, first: str, t, **others) -> int:
+    """The CUDA device that all the given tensors lie on (None is none)."""
+    d = t.get_device()
+    if d < 0:
+        raise RuntimeError(f"x_b200.{what}: {first} must be a CUDA tensor (there is no CPU path)")
+    for name, o in others.items():
+        if o is not None and o.get_device() != d:
+            if not o.is_cuda:
+                raise RuntimeError(f"x_b200.{what}: {name} must be a CUDA tensor (there is no CPU path)")
+            raise RuntimeError(f"x_b200.{what}: {name} lies on {o.device}, {first} on {t.device}")
+    return d
 
 
-def _need_dtype(what: str, name: str, t, dtypes):
-    if t is not None and t.dtype not in dtypes:
-        raise RuntimeError(f"x_b200.{what}: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-
-
-def _on(dev):
-    """The device of the tensors for the launch, if it is not the current one."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _stream(dev):
-    """The current stream of the device as an integer (a Stream object costs several microseconds to make)."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+def _dtype_code(what: str, name: str, t) -> int:
+    code = L.DTYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"x_b200.{what}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
 
 
 def _rows(t):
@@ -67,44 +60,47 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 # ------------------------------------------------------------------------------------------- embedding
 def _embedding_fwd(weight, idx, scale):
+    dev = weight.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _embedding_fwd(weight, idx, scale)
     w, ldw = _rows(weight)
     V, D = w.shape
-    dev = w.device
-    with _on(dev):
-        out = torch.empty(*idx.shape, D, dtype=w.dtype, device=dev)
-        L.check(L.load_library().atlb_embedding_fwd(L.DTYPES[w.dtype], w.data_ptr(), ldw, V, D, idx.data_ptr(),
-                                                    idx.numel(), scale, out.data_ptr(), _stream(dev)), "embedding")
+    out = w.new_empty((*idx.shape, D))
+    L.check(L.load_library().atlb_embedding_fwd(L.DTYPES[w.dtype], w.data_ptr(), ldw, V, D, idx.data_ptr(), idx.numel(),
+                                                scale, out.data_ptr(), _stream(dev)), "embedding")
     return out
+
+
+def _embedding_bwd(g, idx, V, D, scale):
+    dev = g.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _embedding_bwd(g, idx, V, D, scale)
+    N, lib = idx.numel(), L.load_library()
+    g, ldg = _rows(g if g.dim() == 2 else g.reshape(N, D))
+    grad = g.new_empty((V, D))
+    nb = lib.atlb_embedding_workspace_bytes(N, V, D)
+    ws = L.workspace(nb, g.device)
+    L.check(lib.atlb_embedding_bwd(L.DTYPES[g.dtype], g.data_ptr(), ldg, idx.data_ptr(), N, V, D, scale, grad.data_ptr(),
+                                   ws.data_ptr(), nb, _stream(dev)), "embedding_bwd")
+    return grad
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, idx, scale):
         ctx.save_for_backward(idx)
-        ctx.meta = (weight.shape, scale)
+        ctx.meta = (*weight.shape, scale)
         return _embedding_fwd(weight, idx, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         (idx,) = ctx.saved_tensors
-        (V, D), scale = ctx.meta
-        g, ldg = _rows(g.reshape(idx.numel(), D))
-        N = idx.numel()
-        dev, lib = g.device, L.load_library()
-        with _on(dev):
-            grad = torch.empty(V, D, dtype=g.dtype, device=dev)
-            nb = lib.atlb_embedding_workspace_bytes(N, V, D)
-            ws = L.workspace(nb, dev)
-            L.check(lib.atlb_embedding_bwd(L.DTYPES[g.dtype], g.data_ptr(), ldg, idx.data_ptr(), N, V, D, scale,
-                                           grad.data_ptr(), ws.data_ptr(), nb, _stream(dev)), "embedding_bwd")
-        return grad, None, None
+        return _embedding_bwd(g, idx, *ctx.meta), None, None
 
 
 def embedding(weight: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
@@ -114,34 +110,39 @@ def embedding(weight: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> to
     zeros and gives no gradient, as :func:`x_b200.gather` does outside the image: events that left the sensor and
     padding (-1) need no mask.  The gradient of ``weight`` is summed over the events of each row in their order, in
     float32 and without atomics; rows that no event reads get zeros."""
-    _need("embedding", weight=weight, idx=idx)
+    _device("embedding", "weight", weight, idx=idx)
     if weight.dim() != 2:
         raise ValueError(f"x_b200.embedding: weight must be (V, D), got {tuple(weight.shape)}")
-    _need_dtype("embedding", "weight", weight, L.DTYPES)
-    _need_dtype("embedding", "idx", idx, (torch.int64, torch.int32, torch.int16, torch.uint8))
+    _dtype_code("embedding", "weight", weight)
+    if idx.dtype not in _INDEX_TYPES:
+        raise RuntimeError(f"x_b200.embedding: idx must be int64, int32, int16 or uint8, got {idx.dtype}")
     idx = idx.long().contiguous()
-    if _wants_grad(weight):
+    if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(weight, idx, float(scale))
     return _embedding_fwd(weight, idx, float(scale))
 
 
 # ------------------------------------------------------------------------------------------- dropout
 def _dropout_run(x, residual, p, seed, call):
+    """call: an integer, or a device tensor."""
+    dev = x.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _dropout_run(x, residual, p, seed, call)
     x = x.contiguous()
-    dev, dev_call = x.device, call if torch.is_tensor(call) else None
-    with _on(dev):
-        out = torch.empty_like(x)
-        L.check(L.load_library().atlb_dropout(L.DTYPES[x.dtype], x.data_ptr(), _addr(residual), x.numel(), p, seed,
-                                              0 if dev_call is not None else call, _addr(dev_call), out.data_ptr(),
-                                              _stream(dev)), "dropout")
+    out = torch.empty_like(x)
+    call, call_dev = (call, None) if isinstance(call, int) else (0, call.data_ptr())
+    L.check(L.load_library().atlb_dropout(L.DTYPES[x.dtype], x.data_ptr(), _addr(residual), x.numel(), p, seed, call,
+                                          call_dev, out.data_ptr(), _stream(dev)), "dropout")
     return out
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, call):
-        ctx.meta = (p, seed, None if torch.is_tensor(call) else call)
-        ctx.save_for_backward(*([call] if torch.is_tensor(call) else []))
+        ctx.meta = (p, seed, call if isinstance(call, int) else None)
+        if not isinstance(call, int):
+            ctx.save_for_backward(call)
         return _dropout_run(x, residual, p, seed, call)
 
     @staticmethod
@@ -165,8 +166,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, call=0, residual: torch.Tensor
     same mask, and so does every replay of a CUDA graph that captured an integer ``call``.  ``call`` may be a one-element
     int64 tensor on x's device instead, read when the kernel runs: a captured graph that adds to it after its backward
     pass drops anew on every replay."""
-    dev = _need("dropout", x=x, residual=residual)
-    _need_dtype("dropout", "x", x, L.DTYPES)
+    dev = _device("dropout", "x", x, residual=residual)
+    _dtype_code("dropout", "x", x)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"x_b200.dropout: p = {p} lies outside [0, 1]")
     if residual is not None:
@@ -175,32 +176,56 @@ def dropout(x: torch.Tensor, p: float, seed: int, call=0, residual: torch.Tensor
                              f"x {tuple(x.shape)} {x.dtype}")
         residual = residual.contiguous()
     if torch.is_tensor(call):
-        if call.numel() != 1 or call.dtype != torch.int64 or call.device != dev:
+        if call.numel() != 1 or call.dtype != torch.int64 or call.get_device() != dev:
             raise ValueError("x_b200.dropout: call must be an integer or a one-element int64 tensor on x's device")
     else:
         call = int(call) & _MASK64
     seed = int(seed) & _MASK64
-    if _wants_grad(x, residual):
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, residual, float(p), seed, call)
     return _dropout_run(x, residual, float(p), seed, call)
 
 
 # ------------------------------------------------------------------------------------------- recurrence
 def _recurrence_fwd(gate, x, b, B, h0, kind, want_state, save):
+    dev = x.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _recurrence_fwd(gate, x, b, B, h0, kind, want_state, save)
     gate, ldgate = _rows(gate)
     x, ldx = _rows(x)
     N, D = x.shape
-    dev, lib = x.device, L.load_library()
-    with _on(dev):
-        h = torch.empty(N, D, dtype=x.dtype, device=dev)
-        hT = torch.empty(B, D, dtype=torch.float32, device=dev) if want_state else None
-        saved = L.workspace(lib.atlb_recurrence_saved_bytes(N, D), dev) if save else None
-        nb = lib.atlb_recurrence_workspace_bytes(N, D)
-        ws = L.workspace(nb, dev)
-        L.check(lib.atlb_recurrence_fwd(L.DTYPES[x.dtype], kind, gate.data_ptr(), ldgate, x.data_ptr(), ldx, _addr(b),
-                                        N, B, D, _addr(h0), h.data_ptr(), _addr(hT), _addr(saved), ws.data_ptr(), nb,
-                                        _stream(dev)), "linear_recurrence")
+    lib = L.load_library()
+    h = x.new_empty((N, D))
+    hT = x.new_empty((B, D), dtype=torch.float32) if want_state else None
+    saved = L.workspace(lib.atlb_recurrence_saved_bytes(N, D), x.device) if save else None
+    nb = lib.atlb_recurrence_workspace_bytes(N, D)
+    ws = L.workspace(nb, x.device)
+    L.check(lib.atlb_recurrence_fwd(L.DTYPES[x.dtype], kind, gate.data_ptr(), ldgate, x.data_ptr(), ldx, _addr(b), N, B, D,
+                                    _addr(h0), h.data_ptr(), _addr(hT), _addr(saved), ws.data_ptr(), nb, _stream(dev)),
+            "linear_recurrence")
     return h, hT, saved
+
+
+def _recurrence_bwd(gate, x, b, B, h0, kind, saved, gh, ghT):
+    dev = x.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _recurrence_bwd(gate, x, b, B, h0, kind, saved, gh, ghT)
+    gate, ldgate = _rows(gate)
+    x, ldx = _rows(x)
+    gh, ldgh = _rows(torch.zeros_like(x) if gh is None else gh)
+    ghT = None if ghT is None else ghT.contiguous()
+    N, D = x.shape
+    lib = L.load_library()
+    ggate, gx = x.new_empty((N, D)), x.new_empty((N, D))
+    gh0 = x.new_empty((B, D), dtype=torch.float32) if h0 is not None else None
+    nb = lib.atlb_recurrence_workspace_bytes(N, D)
+    ws = L.workspace(nb, x.device)
+    L.check(lib.atlb_recurrence_bwd(L.DTYPES[x.dtype], kind, gate.data_ptr(), ldgate, x.data_ptr(), ldx, _addr(b), N, B, D,
+                                    _addr(h0), saved.data_ptr(), gh.data_ptr(), ldgh, _addr(ghT), ggate.data_ptr(),
+                                    gx.data_ptr(), _addr(gh0), ws.data_ptr(), nb, _stream(dev)), "linear_recurrence_bwd")
+    return ggate, gx, gh0
 
 
 class _Recurrence(torch.autograd.Function):
@@ -217,21 +242,7 @@ class _Recurrence(torch.autograd.Function):
     def backward(ctx, gh, ghT):
         gate, x, b, h0, saved = ctx.saved_tensors
         B, kind = ctx.meta
-        gate, ldgate = _rows(gate)
-        x, ldx = _rows(x)
-        gh, ldgh = _rows(torch.zeros_like(x) if gh is None else gh)
-        ghT = None if ghT is None else ghT.contiguous()
-        N, D = x.shape
-        dev, lib = x.device, L.load_library()
-        with _on(dev):
-            ggate, gx = (torch.empty(N, D, dtype=x.dtype, device=dev) for _ in range(2))
-            gh0 = torch.empty(B, D, dtype=torch.float32, device=dev) if h0 is not None else None
-            nb = lib.atlb_recurrence_workspace_bytes(N, D)
-            ws = L.workspace(nb, dev)
-            L.check(lib.atlb_recurrence_bwd(L.DTYPES[x.dtype], kind, gate.data_ptr(), ldgate, x.data_ptr(), ldx,
-                                            _addr(b), N, B, D, _addr(h0), saved.data_ptr(), gh.data_ptr(), ldgh,
-                                            _addr(ghT), ggate.data_ptr(), gx.data_ptr(), _addr(gh0), ws.data_ptr(), nb,
-                                            _stream(dev)), "linear_recurrence_bwd")
+        ggate, gx, gh0 = _recurrence_bwd(gate, x, b, B, h0, kind, saved, gh, ghT)
         return ggate, gx, None, None, gh0, None, None
 
 
@@ -250,29 +261,32 @@ def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, b: torch.Tensor | Non
     row (default zero).  Returns h (N, D), or (h, state) with ``return_state``: state (B, D) float32 after each
     window's last row (h0 where a window has none), to be given as the next call's ``h0``; one row per window is one
     step.  Differentiable in gate, x and h0, through h and state."""
-    _need("linear_recurrence", x=x, gate=gate, b=b, h0=h0)
-    _need_dtype("linear_recurrence", "x", x, L.DTYPES)
+    _device("linear_recurrence", "x", x, gate=gate, b=b, h0=h0)
+    _dtype_code("linear_recurrence", "x", x)
     if x.dim() != 2 or gate.shape != x.shape or gate.dtype != x.dtype:
         raise ValueError(f"x_b200.linear_recurrence: gate and x must be (N, D) of one dtype, got "
                          f"{tuple(gate.shape)} {gate.dtype} and {tuple(x.shape)} {x.dtype}")
-    if kind not in L.REC_KINDS:
+    code = L.REC_KINDS.get(kind)
+    if code is None:
         raise ValueError(f"x_b200.linear_recurrence: unknown kind {kind!r}")
     N, D = x.shape
     B = int(B)
     if B < 0 or (b is None and (B < 1 or N % B)):
         raise ValueError(f"x_b200.linear_recurrence: {N} rows do not make {B} equal windows")
     if b is not None:
-        _need_dtype("linear_recurrence", "b", b, (torch.int64,))
+        if b.dtype != torch.int64:
+            raise RuntimeError(f"x_b200.linear_recurrence: b must be int64, got {b.dtype}")
         if b.shape != (N,):
             raise ValueError(f"x_b200.linear_recurrence: b must be ({N},), got {tuple(b.shape)}")
         b = b.contiguous()
     if h0 is not None:
-        _need_dtype("linear_recurrence", "h0", h0, (torch.float32,))
+        if h0.dtype != torch.float32:
+            raise RuntimeError(f"x_b200.linear_recurrence: h0 must be float32, got {h0.dtype}")
         if h0.shape != (B, D):
             raise ValueError(f"x_b200.linear_recurrence: h0 must be ({B}, {D}), got {tuple(h0.shape)}")
         h0 = h0.contiguous()
-    if _wants_grad(gate, x, h0):
-        h, state = _Recurrence.apply(gate, x, b, B, h0, L.REC_KINDS[kind], return_state)
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+        h, state = _Recurrence.apply(gate, x, b, B, h0, code, return_state)
     else:
-        h, state, _ = _recurrence_fwd(gate, x, b, B, h0, L.REC_KINDS[kind], return_state, False)
+        h, state, _ = _recurrence_fwd(gate, x, b, B, h0, code, return_state, False)
     return (h, state) if return_state else h

@@ -80,6 +80,18 @@ __device__ __forceinline__ Pair sort_pair(const void* src, long long i, unsigned
   return Pair{q.x, q.y};
 }
 
+// Zeros, by all threads of the CTAs that call it.
+__device__ __forceinline__ void write_zeros(char* dst, long long bytes) {
+  const long long vecs = bytes / 16, step = (long long)gridDim.x * kSortThreads;
+  const long long i0 = blockIdx.x * (long long)kSortThreads + threadIdx.x;
+  if (reinterpret_cast<uintptr_t>(dst) % 16 == 0) {
+    for (long long i = i0; i < vecs; i += step) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
+    if (i0 < bytes % 16) dst[vecs * 16 + i0] = 0;
+  } else {
+    for (long long i = i0; i < bytes / 2; i += step) reinterpret_cast<unsigned short*>(dst)[i] = 0;
+  }
+}
+
 template <bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) k_sort_count(const void* __restrict__ src, long long N, unsigned V,
                                                              int shift, int bins, int tiles,
@@ -87,16 +99,7 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_count(const void* __restr
                                                              long long grad_bytes) {
   __shared__ unsigned hist[kMaxBins];
   // on the way, and in CTAs of their own behind the tiles: the gradient starts as zeros (rows that no pair names)
-  if (FIRST) {
-    const long long vecs = grad_bytes / 16, step = (long long)gridDim.x * kSortThreads;
-    const long long i0 = blockIdx.x * (long long)kSortThreads + threadIdx.x;
-    if (reinterpret_cast<uintptr_t>(grad) % 16 == 0) {
-      for (long long i = i0; i < vecs; i += step) reinterpret_cast<uint4*>(grad)[i] = make_uint4(0, 0, 0, 0);
-      if (i0 < grad_bytes % 16) grad[vecs * 16 + i0] = 0;
-    } else {
-      for (long long i = i0; i < grad_bytes / 2; i += step) reinterpret_cast<unsigned short*>(grad)[i] = 0;
-    }
-  }
+  if (FIRST) write_zeros(grad, grad_bytes);
   if (blockIdx.x >= tiles) return;
   for (int d = threadIdx.x; d < bins; d += kSortThreads) hist[d] = 0;
   __syncthreads();
@@ -182,27 +185,89 @@ __global__ void __launch_bounds__(kScanDigits * kScanRuns) k_sort_scan(unsigned*
   }
 }
 
-// Stable placement: a warp ranks 32 neighbouring pairs at a time among equal digits (match), on top of the counts
-// of the rounds and warps before it.  The tile is put in order in shared memory first, so that pairs of one digit leave
-// side by side (4M pairs of 33 rows 34 us, scattered one by one 37).
+// The order of one tile by a digit, stable.  A warp ranks 32 neighbouring pairs at a time among equal digits (match), on
+// top of the counts of the rounds and warps before it; the pairs then stand in order in shared memory.
+template <int ITEMS>
+struct TileSort {
+  static constexpr int kTile = kSortThreads * ITEMS;
+  union {
+    unsigned short hist[kSortWarps][kMaxBins];
+    uint2 pair[kTile];  // in order, once the counts are not needed any more
+  };
+  unsigned local[kMaxBins];  // where each digit's pairs begin
+  unsigned sm[kSortWarps];
+
+  // Pair r of a thread is the tile's number wid * 32 * ITEMS + r * 32 + lane; the first n of the tile's exist.  Ends with
+  // a barrier.
+  __device__ __forceinline__ void order(const Pair (&p)[ITEMS], int n, int shift, int bins) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, first = wid * (32 * ITEMS) + lane;
+    for (int d = lane; d < bins; d += 32) hist[wid][d] = 0;
+    __syncwarp();
+    unsigned at[ITEMS];  // rank among the warp's pairs of the digit, then the place in the tile
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+      const bool in = first + r * 32 < n;
+      const unsigned d = in ? (p[r].row >> shift) & (bins - 1) : 0xffffffffu;
+      const unsigned peers = __match_any_sync(0xffffffffu, d);
+      const unsigned before = in ? hist[wid][d] : 0;
+      __syncwarp();
+      at[r] = before + __popc(peers & ((1u << lane) - 1));
+      if (in && lane == __ffs(peers) - 1) hist[wid][d] = (unsigned short)(before + __popc(peers));
+      __syncwarp();
+    }
+    __syncthreads();
+    unsigned carry = 0;
+    for (int d0 = 0; d0 < bins; d0 += kSortThreads) {
+      const int d = d0 + threadIdx.x;
+      unsigned c = 0, total;
+      if (d < bins) {
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+          const unsigned h = hist[w][d];
+          hist[w][d] = (unsigned short)c;
+          c += h;
+        }
+      }
+      const unsigned ex = block_scan<kSortThreads>(c, sm, &total);
+      if (d < bins) local[d] = carry + ex;
+      carry += total;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+      if (first + r * 32 < n) {
+        const unsigned d = (p[r].row >> shift) & (bins - 1);
+        at[r] += local[d] + hist[wid][d];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+      if (first + r * 32 < n) pair[at[r]] = make_uint2(p[r].row, p[r].event);
+    __syncthreads();
+  }
+};
+
+// Placement of the tiles' pairs.  They leave in the tile's order, so that pairs of one digit leave side by side (4M pairs
+// of 33 rows 34 us, scattered one by one 37).
 template <bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restrict__ src, long long N, unsigned V,
                                                              int shift, int bins, int tiles,
                                                              const unsigned* __restrict__ counts,
                                                              const unsigned* __restrict__ totals,
                                                              uint2* __restrict__ out) {
-  constexpr int kTile = kSortThreads * ITEMS;
-  static_assert(kTile * sizeof(uint2) <= sizeof(unsigned short) * kSortWarps * kMaxBins, "the pairs reuse the counts");
-  __shared__ __align__(8) unsigned short hist[kSortWarps][kMaxBins];
-  __shared__ unsigned start[kMaxBins], local[kMaxBins];
-  __shared__ unsigned sm[kSortWarps];
+  using Tile = TileSort<ITEMS>;
+  __shared__ Tile ts;
+  __shared__ unsigned start[kMaxBins];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const long long tile0 = blockIdx.x * (long long)kTile, base = tile0 + wid * (32 * ITEMS) + lane;
+  const long long tile0 = blockIdx.x * (long long)Tile::kTile;
+  const int n = N - tile0 < Tile::kTile ? (int)(N - tile0) : Tile::kTile;
   Pair p[ITEMS];
 #pragma unroll
-  for (int r = 0; r < ITEMS; ++r)
-    if (base + r * 32 < N) p[r] = sort_pair<FIRST>(src, base + r * 32, V);
-  for (int d = lane; d < bins; d += 32) hist[wid][d] = 0;
+  for (int r = 0; r < ITEMS; ++r) {
+    const int i = wid * (32 * ITEMS) + r * 32 + lane;
+    if (i < n) p[r] = sort_pair<FIRST>(src, tile0 + i, V);
+  }
   unsigned carry = 0;
   for (int d0 = 0; d0 < bins; d0 += kSortThreads) {
     const int d = d0 + threadIdx.x;
@@ -220,67 +285,45 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_place(const void* __restr
         }
       }
     }
-    const unsigned ex = block_scan<kSortThreads>(all, sm, &total);
+    const unsigned ex = block_scan<kSortThreads>(all, ts.sm, &total);
     if (d < bins) start[d] = carry + ex + before;
     carry += total;
   }
-  unsigned at[ITEMS];  // lanes of the same digit, then the rank among the warp's pairs of it, then the place in the tile
-#pragma unroll
-  for (int r = 0; r < ITEMS; ++r)
-    at[r] = __match_any_sync(0xffffffffu, base + r * 32 < N ? (p[r].row >> shift) & (bins - 1) : 0xffffffffu);
-#pragma unroll
-  for (int r = 0; r < ITEMS; ++r) {
-    const bool in = base + r * 32 < N;
-    const unsigned d = in ? (p[r].row >> shift) & (bins - 1) : 0, peers = at[r];
-    const unsigned before = in ? hist[wid][d] : 0;
-    __syncwarp();
-    at[r] = before + __popc(peers & ((1u << lane) - 1));
-    if (in && lane == __ffs(peers) - 1) hist[wid][d] = (unsigned short)(before + __popc(peers));
-    __syncwarp();
-  }
-  __syncthreads();
-  carry = 0;
-  for (int d0 = 0; d0 < bins; d0 += kSortThreads) {
-    const int d = d0 + threadIdx.x;
-    unsigned c = 0, total;
-    if (d < bins) {
-#pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) {
-        const unsigned h = hist[w][d];
-        hist[w][d] = (unsigned short)c;
-        c += h;
-      }
-    }
-    const unsigned ex = block_scan<kSortThreads>(c, sm, &total);
-    if (d < bins) {
-      local[d] = carry + ex;
-      start[d] -= carry + ex;
-    }
-    carry += total;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int r = 0; r < ITEMS; ++r) {
-    if (base + r * 32 < N) {
-      const unsigned d = (p[r].row >> shift) & (bins - 1);
-      at[r] += local[d] + hist[wid][d];
-    }
-  }
-  __syncthreads();
-  uint2* tile = reinterpret_cast<uint2*>(hist);
-#pragma unroll
-  for (int r = 0; r < ITEMS; ++r)
-    if (base + r * 32 < N) tile[at[r]] = make_uint2(p[r].row, p[r].event);
-  __syncthreads();
-  const int n = N - tile0 < kTile ? (int)(N - tile0) : kTile;
+  ts.order(p, n, shift, bins);
 #pragma unroll
   for (int r = 0; r < ITEMS; ++r) {
     const int i = r * kSortThreads + threadIdx.x;
     if (i < n) {
-      const uint2 q = tile[i];
-      out[start[(q.x >> shift) & (bins - 1)] + i] = q;
+      const uint2 q = ts.pair[i];
+      const unsigned d = (q.x >> shift) & (bins - 1);
+      out[start[d] - ts.local[d] + i] = q;
     }
   }
+}
+
+// One tile: all passes in one CTA, the pairs in shared memory between them; the CTAs behind it write zeros.
+constexpr int kSmallItems = 8;
+__global__ void __launch_bounds__(kSortThreads) k_sort_small(const long long* __restrict__ idx, int n, unsigned V, int passes,
+                                                             int bits, uint2* __restrict__ out, char* __restrict__ grad,
+                                                             long long grad_bytes) {
+  __shared__ TileSort<kSmallItems> ts;
+  write_zeros(grad, grad_bytes);
+  if (blockIdx.x > 0) return;
+  const int first = (threadIdx.x >> 5) * (32 * kSmallItems) + (threadIdx.x & 31);
+  Pair p[kSmallItems];
+#pragma unroll
+  for (int r = 0; r < kSmallItems; ++r)
+    if (first + r * 32 < n) p[r] = sort_pair<true>(idx, first + r * 32, V);
+  for (int k = 0; k < passes; ++k) {
+    if (k > 0) {
+#pragma unroll
+      for (int r = 0; r < kSmallItems; ++r)
+        if (first + r * 32 < n) p[r] = Pair{ts.pair[first + r * 32].x, ts.pair[first + r * 32].y};
+      __syncthreads();
+    }
+    ts.order(p, n, k * bits, 1 << bits);
+  }
+  for (int i = threadIdx.x; i < n; i += kSortThreads) out[i] = ts.pair[i];
 }
 
 struct SortPlan {
@@ -510,15 +553,21 @@ int embedding_bwd(int dtype, const void* g, long long ldg, const long long* idx,
   const EmbedWs w = carve(ws, N, V, D);
   const int bins = 1 << p.bits, L = sum_chunk(N, D);
   const void* src = idx;
-  for (int i = 0; i < p.passes; ++i) {
+  // enough CTAs to write the zeros as well: 64 KB each, up to two per SM
+  const int zero = (int)(grad_bytes / 65536 < 296 ? grad_bytes / 65536 : 296);
+  const bool small = N <= TileSort<kSmallItems>::kTile;
+  if (small) {
+    launch(k_sort_small, zero > 1 ? zero : 1, kSortThreads, 0, s, idx, (int)N, (unsigned)V, p.passes, p.bits, w.pair[0],
+           (char*)grad, (long long)grad_bytes);
+    src = w.pair[0];
+  }
+  for (int i = 0; !small && i < p.passes; ++i) {
     uint2* dst = w.pair[i & 1];
     auto pass = [&](auto first, auto items) {
       constexpr bool F = decltype(first)::value;
       constexpr int I = decltype(items)::value;
-      // enough CTAs to write the zeros as well: 64 KB each, up to two per SM
-      const int zero = F ? (int)(grad_bytes / 65536 < 296 ? grad_bytes / 65536 : 296) : 0;
-      launch(k_sort_count<F, I>, p.tiles > zero ? p.tiles : zero, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits, bins,
-             p.tiles, w.counts, (char*)grad, (long long)grad_bytes);
+      launch(k_sort_count<F, I>, F && zero > p.tiles ? zero : p.tiles, kSortThreads, 0, s, src, N, (unsigned)V, i * p.bits,
+             bins, p.tiles, w.counts, (char*)grad, (long long)grad_bytes);
       if (p.tiles > kFewTiles)
         launch(k_sort_scan, (bins + kScanDigits - 1) / kScanDigits, kScanDigits * kScanRuns, 0, s, w.counts, bins,
                p.tiles, w.totals);

@@ -84,9 +84,9 @@ def dropout(x, p, seed, call, residual=None):
 
 # ------------------------------------------------------------------------------------------------ recurrence
 def sigmoid_error(kind, zmax):
-    """Relative error of a and 1 - a, in U.  sigmoid: exp(-|z|) by __expf, 2 + 1.173 |z| ulp, then 1 + e, the quotient
-    (__fdividef, 2 ulp) and the product; an ulp is at most 2 U of the value."""
-    return 2 * (2 + np.floor(1.173 * zmax)) + 1 + 4 + 1 if kind == "sigmoid" else 0.0
+    """Relative error of a and 1 - a, in U.  sigmoid: exp(-|z|), at worst by __expf with 2 + 1.173 |z| ulp, then 1 + e, its
+    reciprocal (1 ulp) and the product; an ulp is at most 2 U of the value."""
+    return 2 * (2 + np.floor(1.173 * zmax)) + 1 + 2 + 1 if kind == "sigmoid" else 0.0
 
 
 def recurrence(kind, gate, x, b, B, h0=None, gh=None, ghT=None, xerr=0.0, zmax=None):

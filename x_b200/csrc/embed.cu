@@ -400,6 +400,15 @@ __global__ void __launch_bounds__(kThreads, 3) k_embed_sum(const T* __restrict__
       const int m = j + kAhead + q;
       next[q] = m < j1 ? __ldg(pair + m) : make_uint2(V, 0);
     }
+    // all of the run, as most are where runs are long: summed among themselves first (the pairs are sorted, so the last
+    // row tells), a quarter of the roundings on the way
+    static_assert(kAhead == 4, "four rows at a time");
+    if (row[0] == cur && row[3] == cur) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        acc[e] += (to_f32(r[0].v[e]) + to_f32(r[1].v[e])) + (to_f32(r[2].v[e]) + to_f32(r[3].v[e]));
+      continue;
+    }
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       if (j + q < j1 && row[q] != cur) {
@@ -420,14 +429,15 @@ __global__ void __launch_bounds__(kThreads, 3) k_embed_sum(const T* __restrict__
 
 // The chunk in which a run over several chunks begins joins its partial sums.  A CTA looks after 32 chunks: a warp each
 // for the runs that go on over fewer than 32 more chunks, in order; then, for a longer one, all its threads, 64 rows of
-// them over 16 columns: each takes every 64th partial sum, and these are added in order.
+// them over 16 columns: each takes every 64th partial sum, and these are added in order.  The few sums of sums are taken
+// in 64 bits, which costs nothing here and keeps long runs at the error of their chunks.
 constexpr int kJoinThreads = 1024, kLongCols = 16, kLongRows = kJoinThreads / kLongCols;
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) k_embed_join(const uint2* __restrict__ pair, int N, unsigned V, int D,
                                                              int L, unsigned chunks, float scale,
                                                              const float* __restrict__ part, T* __restrict__ grad) {
-  __shared__ float sm[kLongRows][kLongCols + 1];
+  __shared__ double sm[kLongRows][kLongCols + 1];
   __shared__ unsigned long_row[32];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const unsigned chunk = blockIdx.x * 32 + wid;
@@ -446,10 +456,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_embed_join(const uint2* __rest
     if (!is_long && blockIdx.y == 0) {
       const unsigned last = chunk + __ffs(ends);
       for (int c = lane; c < D; c += 32) {
-        float acc = part[((long long)chunk * 2 + 1) * D + c];
+        double acc = part[((long long)chunk * 2 + 1) * D + c];
 #pragma unroll 4
         for (unsigned e = chunk + 1; e <= last; ++e) acc += part[(long long)e * 2 * D + c];
-        grad[(long long)row * D + c] = from_f32<T>(acc * scale);
+        grad[(long long)row * D + c] = from_f32<T>((float)acc * scale);
       }
     }
   }
@@ -468,7 +478,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_embed_join(const uint2* __rest
     }
     for (int c0 = blockIdx.y * kLongCols; c0 < D; c0 += gridDim.y * kLongCols) {
       const int c = c0 + x;
-      float acc = 0.f;
+      double acc = 0.0;
       if (c < D) {
         if (y == 0) acc = part[((long long)from * 2 + 1) * D + c];
 #pragma unroll 8
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_embed_join(const uint2* __rest
       if (y == 0 && c < D) {
 #pragma unroll 8
         for (int k = 1; k < kLongRows; ++k) acc += sm[k][x];
-        grad[(long long)r * D + c] = from_f32<T>(acc * scale);
+        grad[(long long)r * D + c] = from_f32<T>((float)acc * scale);
       }
       __syncthreads();
     }

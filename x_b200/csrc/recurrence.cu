@@ -73,22 +73,89 @@ __device__ __forceinline__ void row_terms(T gate, T in, float* a, float* w, floa
 }
 
 // ------------------------------------------------------------------------------------------------ maps
-// The map of some rows in one column; cut: they hold a window's border, so the state before them does not matter.
+// The map h -> A h + C of some rows in one column; cut: they hold a window's border, so the state before them does not
+// matter.  C is the state that a zero leaves behind, no larger than the magnitudes that the rows themselves go through.
+// A has no such bound.  Sigmoid: a product of values in [0, 1], which may at worst vanish; plain fp32 (below 2^-149 over a
+// group, a state before it counts as zero).
 struct Map {
   float A, C;
   bool cut;
+  __device__ __forceinline__ static Map identity() { return Map{1.f, 0.f, false}; }
 };
-__device__ __forceinline__ Map identity() { return Map{1.f, 0.f, false}; }
-// A zero state leaves C: the product of many gates above one may overflow.
-__device__ __forceinline__ float apply(const Map& m, float s) { return m.cut || s == 0.f ? m.C : fmaf(m.A, s, m.C); }
+__device__ __forceinline__ float apply(const Map& m, float s) { return m.cut ? m.C : fmaf(m.A, s, m.C); }
 __device__ __forceinline__ Map then(const Map& a, const Map& b) { return Map{a.A * b.A, apply(b, a.C), a.cut || b.cut}; }
 
-// As 64 bits: A below, C above; a cut stands in the place of A, as a NaN that arithmetic does not make.
-constexpr unsigned kCut = 0x7fc00c07u, kNan = 0x7fffffffu;
-__device__ __forceinline__ uint2 pack_map(const Map& m) {
-  return make_uint2(m.cut ? kCut : (m.A != m.A ? kNan : __float_as_uint(m.A)), __float_as_uint(m.C));
+// Decay: gates of any size.  A product over a chunk may leave fp32's range where no state does (130 gates of 2 and 130 of
+// 1/2 behind a state of 0.01), so A = m 2^e with |m| in [1, 2), or m zero, infinite or NaN.  Device time of 1M bf16 rows of
+// 64 columns, both ways: 364 us, where plain fp32 products took 349; 100k fp32 rows of 32: 48 and 45.
+struct WideMap {
+  float m, C;
+  int e;
+  bool cut;
+  __device__ __forceinline__ static WideMap identity() { return WideMap{1.f, 0.f, 0, false}; }
+};
+constexpr int kMaxExp = 32000;  // more makes no difference: beyond 2^+-278 a state vanishes or overflows in any case
+__device__ __forceinline__ int clamp_to(int e, int most) { return max(-most, min(most, e)); }
+// 2^k for -127 < k < 128; 0 for -127.
+__device__ __forceinline__ float power2(int k) { return __int_as_float((k + 127) << 23); }
+// Half of 2^e goes to the state and half to m: neither leaves fp32's range where the product does not.
+__device__ __forceinline__ float apply(const WideMap& w, float s) {
+  const int e = clamp_to(w.e, 254), half = e >> 1;
+  return w.cut ? w.C : fmaf(w.m * power2(e - half), s * power2(half), w.C);
 }
-__device__ __forceinline__ Map unpack_map(uint2 v) { return Map{__uint_as_float(v.x), __uint_as_float(v.y), v.x == kCut}; }
+__device__ __forceinline__ WideMap then(const WideMap& a, const WideMap& b) {
+  const float m = a.m * b.m;
+  const bool two = fabsf(m) >= 2.f;
+  return WideMap{two ? 0.5f * m : m, apply(b, a.C), clamp_to(a.e + b.e + two, kMaxExp), a.cut || b.cut};
+}
+// v = m 2^e
+__device__ __forceinline__ void split(float v, float* m, int* e) {
+  const bool small = fabsf(v) < 0x1p-126f;  // zero or subnormal
+  const unsigned b = __float_as_uint(small ? v * 0x1p64f : v);
+  const int x = b >> 23 & 255;
+  const bool plain = x != 255 && v != 0.f;
+  *m = plain ? __uint_as_float((b & 0x807fffffu) | 0x3f800000u) : v;
+  *e = plain ? x - (small ? 191 : 127) : 0;
+}
+
+// Arrays of maps: A and C as 64 bits (a cut stands in the place of A, as a NaN that arithmetic does not make), or m and C
+// with e beside them (kCutExp for a cut).
+constexpr unsigned kCut = 0x7fc00c07u, kNan = 0x7fffffffu;
+constexpr short kCutExp = SHRT_MIN;
+struct Maps {
+  uint2* ac;
+  short* e;
+  __device__ __forceinline__ void put(long long i, const Map& m) const {
+    ac[i] = make_uint2(m.cut ? kCut : (m.A != m.A ? kNan : __float_as_uint(m.A)), __float_as_uint(m.C));
+  }
+  __device__ __forceinline__ void put(long long i, const WideMap& m) const {
+    ac[i] = make_uint2(__float_as_uint(m.m), __float_as_uint(m.C));
+    e[i] = m.cut ? kCutExp : (short)m.e;
+  }
+};
+__device__ __forceinline__ void unpack(uint2 v, short, Map& m) {
+  m = Map{__uint_as_float(v.x), __uint_as_float(v.y), v.x == kCut};
+}
+__device__ __forceinline__ void unpack(uint2 v, short e, WideMap& m) {
+  m = WideMap{__uint_as_float(v.x), __uint_as_float(v.y), e, e == kCutExp};
+}
+template <typename M>
+constexpr bool kHasExp = std::is_same<M, WideMap>::value;
+template <typename M>  // from shared memory
+__device__ __forceinline__ M map_at(const Maps& a, int i) {
+  M m;
+  unpack(a.ac[i], kHasExp<M> ? a.e[i] : 0, m);
+  return m;
+}
+template <typename M>  // from an earlier kernel's array
+__device__ __forceinline__ M map_of(const Maps& a, long long i) {
+  M m;
+  unpack(__ldg(a.ac + i), kHasExp<M> ? __ldg(a.e + i) : 0, m);
+  return m;
+}
+
+template <int KIND>
+using MapOf = std::conditional_t<KIND == ATLB_REC_DECAY, WideMap, Map>;
 
 // ------------------------------------------------------------------------------------------------ windows
 // Bit r of each word stands for row r of the group: `first` / `last` of its window, `none` when it belongs to no window
@@ -160,16 +227,20 @@ constexpr int kAhead = 4;  // rows in flight per thread
 
 template <typename T, int E, int KIND, bool BWD>
 __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate, Src<T> in, const float* __restrict__ s0,
-                                                      uint2* __restrict__ prefix, uint2* __restrict__ chunk) {
-  __shared__ uint2 sm[kThreads * E];
-  __shared__ uint2 seg[32 * E];  // segments x columns: 16 E, or 32 E where a warp takes a row
+                                                      Maps prefix, Maps chunk) {
+  using M = MapOf<KIND>;
+  constexpr bool kWide = KIND == ATLB_REC_DECAY;
+  constexpr int kSegs = 32 * E;  // segments x columns: 16 E, or 32 E where a warp takes a row
+  __shared__ uint2 sm_ac[kThreads * E], seg_ac[kSegs];
+  __shared__ short sm_e[kWide ? kThreads * E : 1], seg_e[kWide ? kSegs : 1];
+  const Maps sm{sm_ac, sm_e}, seg{seg_ac, seg_e};
   const int sub = threadIdx.x & (S.lanes - 1), per = kThreads / S.lanes, mine = threadIdx.x / S.lanes;
   const int W = S.lanes * E, c = blockIdx.y * W + sub * E, warp_groups = S.lanes >= 32 ? 1 : 32 / S.lanes;
   const long long g = blockIdx.x * (long long)per + mine, r0 = g * kGroup;
   const bool col = c < S.D;
   const Edges ed = group_edges(S, g - mine % warp_groups, warp_groups, mine % warp_groups);
   const unsigned edge = (BWD ? ed.last : ed.first) | ed.none;
-  float A[E], s[E];
+  float A[E], s[E], hi = 1.f, lo = 1.f;  // hi, lo: the largest and the smallest magnitude that A went through
 #pragma unroll
   for (int e = 0; e < E; ++e) { A[e] = 1.f; s[e] = 0.f; }
   auto rows = [&](auto plain) {
@@ -202,6 +273,10 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
           row_terms<KIND>(gp[j].v[e], ip[j].v[e], &a, &w, &v);
           s[e] = BWD ? a * (to_f32(ip[j].v[e]) + s[e]) : fmaf(a, s[e], v);
           A[e] *= a;
+          if (kWide) {
+            hi = fmaxf(hi, fabsf(A[e]));
+            lo = fminf(lo, fabsf(A[e]));
+          }
         }
       }
     }
@@ -212,35 +287,58 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
     rows(std::true_type());
   // joined along the walk, per column: kSeg groups by one thread, then the segments, then the groups again
   const int at = BWD ? per - 1 - mine : mine, segs = (per + kSeg - 1) / kSeg;
+  // A product that left the normal numbers, or came near: the gates once more, their exponents summed apart.  Without a
+  // border the group's rows all exist.
+  const bool far = kWide && edge == 0 && col && !(hi <= 0x1p100f && lo >= 0x1p-100f);
 #pragma unroll
-  for (int e = 0; e < E; ++e) sm[at * W + sub * E + e] = pack_map(Map{A[e], s[e], edge != 0});
+  for (int e = 0; e < E; ++e) {
+    if constexpr (kWide) {
+      WideMap m{A[e], s[e], 0, edge != 0};
+      if (far) {
+        m.m = 1.f;
+#pragma unroll 1
+        for (int r = 0; r < kGroup; ++r) {
+          WideMap row{0.f, 0.f, 0, false};
+          split(to_f32(gate.p[(r0 + r) * gate.ld + c + e]), &row.m, &row.e);
+          m.m *= row.m;
+          m.e += row.e;
+        }
+      }
+      int x;
+      split(m.m, &m.m, &x);
+      m.e += x;
+      sm.put(at * W + sub * E + e, m);
+    } else {
+      sm.put(at * W + sub * E + e, Map{A[e], s[e], edge != 0});
+    }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < segs * W; i += kThreads) {
     const int x = i % W, k0 = i / W * kSeg;
-    Map m = identity();
+    M m = M::identity();
     for (int k = k0; k < k0 + kSeg && k < per; ++k) {
-      const Map next = unpack_map(sm[k * W + x]);
-      sm[k * W + x] = pack_map(m);
+      const M next = map_at<M>(sm, k * W + x);
+      sm.put(k * W + x, m);
       m = then(m, next);
     }
-    seg[i] = pack_map(m);
+    seg.put(i, m);
   }
   __syncthreads();
   for (int x = threadIdx.x; x < W; x += kThreads) {
-    Map m = identity();
+    M m = M::identity();
     for (int k = 0; k < segs; ++k) {
-      const Map next = unpack_map(seg[k * W + x]);
-      seg[k * W + x] = pack_map(m);
+      const M next = map_at<M>(seg, k * W + x);
+      seg.put(k * W + x, m);
       m = then(m, next);
     }
-    if (blockIdx.y * W + x < S.D) chunk[blockIdx.x * (long long)S.D + blockIdx.y * W + x] = pack_map(m);
+    if (blockIdx.y * W + x < S.D) chunk.put(blockIdx.x * (long long)S.D + blockIdx.y * W + x, m);
   }
   __syncthreads();
   if (col && g < S.groups) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      prefix[g * S.D + c + e] =
-          pack_map(then(unpack_map(seg[at / kSeg * W + sub * E + e]), unpack_map(sm[at * W + sub * E + e])));
+      prefix.put(g * S.D + c + e,
+                 then(map_at<M>(seg, at / kSeg * W + sub * E + e), map_at<M>(sm, at * W + sub * E + e)));
   }
 }
 
@@ -252,46 +350,53 @@ __device__ __forceinline__ Map map_above(const Map& m, int by) {
   return Map{__shfl_up_sync(0xffffffffu, m.A, by), __shfl_up_sync(0xffffffffu, m.C, by),
              (bool)__shfl_up_sync(0xffffffffu, (int)m.cut, by)};
 }
+__device__ __forceinline__ WideMap map_above(const WideMap& m, int by) {
+  return WideMap{__shfl_up_sync(0xffffffffu, m.m, by), __shfl_up_sync(0xffffffffu, m.C, by),
+                 __shfl_up_sync(0xffffffffu, m.e, by)};
+}
 // The map of the runs before this thread's in its warp (lanes of one column are kChainCols apart); m becomes the map up
 // to its own.
-__device__ __forceinline__ Map warp_join(Map& m, int lane) {
+template <typename M>
+__device__ __forceinline__ M warp_join(M& m, int lane) {
 #pragma unroll
   for (int by = kChainCols; by < 32; by *= 2) {
-    const Map p = map_above(m, by);
+    const M p = map_above(m, by);
     if (lane >= by) m = then(p, m);
   }
-  const Map before = map_above(m, kChainCols);
-  return lane < kChainCols ? identity() : before;
+  const M before = map_above(m, kChainCols);
+  return lane < kChainCols ? M::identity() : before;
 }
 
-template <bool BWD>
-__global__ void __launch_bounds__(kChainCols * kChainSegs) k_rec_chain(const uint2* __restrict__ chunk, int chunks, int D,
+template <typename M, bool BWD>
+__global__ void __launch_bounds__(kChainCols * kChainSegs) k_rec_chain(Maps chunk, int chunks, int D,
                                                                        float* __restrict__ state) {
   constexpr int kWarps = kChainCols * kChainSegs / 32, kEach = kWarps * kChainCols / 32;
-  __shared__ uint2 sm[kWarps][kChainCols];
+  __shared__ uint2 sm_ac[kWarps * kChainCols];
+  __shared__ short sm_e[kWarps * kChainCols];
   __shared__ float in[kWarps][kChainCols];
+  const Maps sm{sm_ac, sm_e};
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int x = threadIdx.x % kChainCols, sg = threadIdx.x / kChainCols, c = blockIdx.x * kChainCols + x;
   const int run = (chunks + kChainSegs - 1) / kChainSegs, k0 = sg * run, k1 = min(k0 + run, chunks);
   auto at = [&](int k) { return (long long)(BWD ? chunks - 1 - k : k) * D + c; };
-  Map m = identity();
+  M m = M::identity();
   if (c < D) {
 #pragma unroll 8
-    for (int k = k0; k < k1; ++k) m = then(m, unpack_map(chunk[at(k)]));
+    for (int k = k0; k < k1; ++k) m = then(m, map_of<M>(chunk, at(k)));
   }
-  const Map before = warp_join(m, lane);
-  if (lane >= 32 - kChainCols) sm[wid][x] = pack_map(m);
+  const M before = warp_join(m, lane);
+  if (lane >= 32 - kChainCols) sm.put(wid * kChainCols + x, m);
   __syncthreads();
   if (wid == 0) {
     const int w0 = lane / kChainCols * kEach;
-    Map t = identity();
+    M t = M::identity();
 #pragma unroll
-    for (int w = 0; w < kEach; ++w) t = then(t, unpack_map(sm[w0 + w][x]));
+    for (int w = 0; w < kEach; ++w) t = then(t, map_at<M>(sm, (w0 + w) * kChainCols + x));
     float s = apply(warp_join(t, lane), 0.f);
 #pragma unroll
     for (int w = 0; w < kEach; ++w) {
       in[w0 + w][x] = s;
-      s = apply(unpack_map(sm[w0 + w][x]), s);
+      s = apply(map_at<M>(sm, (w0 + w) * kChainCols + x), s);
     }
   }
   __syncthreads();
@@ -299,21 +404,21 @@ __global__ void __launch_bounds__(kChainCols * kChainSegs) k_rec_chain(const uin
   float s = apply(before, in[wid][x]);
 #pragma unroll 8
   for (int k = k0; k < k1; ++k) {
-    const uint2 v = chunk[at(k)];
+    const M next = map_of<M>(chunk, at(k));
     state[at(k)] = s;
-    s = apply(unpack_map(v), s);
+    s = apply(next, s);
   }
 }
 
 // The state that enters group g: the chunk's, through the map from there.  per: groups of a chunk.
-template <int E>
-__device__ __forceinline__ void group_state(const RecShape& S, const uint2* prefix, const float* state, long long g,
+template <typename M, int E>
+__device__ __forceinline__ void group_state(const RecShape& S, const Maps& prefix, const float* state, long long g,
                                             int per, int c, bool in, float (&s)[E]) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     s[e] = 0.f;
     if (in && S.linked)
-      s[e] = apply(unpack_map(prefix[g * S.D + c + e]), S.chunks > 1 ? state[g / per * S.D + c + e] : 0.f);
+      s[e] = apply(map_of<M>(prefix, g * S.D + c + e), S.chunks > 1 ? state[g / per * S.D + c + e] : 0.f);
   }
 }
 
@@ -321,8 +426,7 @@ __device__ __forceinline__ void group_state(const RecShape& S, const uint2* pref
 // 1M rows of 64 bf16 columns: 77 us, 430 MB with the kept states (5.6 TB/s); 4M rows without them 234 us (6.7 TB/s).
 template <typename T, int E, int KIND>
 __global__ void __launch_bounds__(kThreads, 5) k_rec_fwd(RecShape S, Src<T> gate, Src<T> x, const float* __restrict__ h0,
-                                                      const uint2* __restrict__ prefix,
-                                                      const float* __restrict__ state, T* __restrict__ h,
+                                                      Maps prefix, const float* __restrict__ state, T* __restrict__ h,
                                                       float* __restrict__ hT, float* __restrict__ saved) {
   const int sub = threadIdx.x & (S.lanes - 1), per = kThreads / S.lanes, mine = threadIdx.x / S.lanes;
   const int c = (blockIdx.y * S.lanes + sub) * E, warp_groups = S.lanes >= 32 ? 1 : 32 / S.lanes;
@@ -332,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_rec_fwd(RecShape S, Src<T> gate
   const Edges ed = group_edges(S, g - mine % warp_groups, warp_groups, mine % warp_groups);
   const unsigned edge = ed.first | ed.none;
   float s[E];
-  group_state(S, prefix, state, g, per, c, col && g < S.groups, s);
+  group_state<MapOf<KIND>>(S, prefix, state, g, per, c, col && g < S.groups, s);
   auto rows = [&](auto plain) {
     const T *pg = gate.p + r0 * gate.ld + (col ? c : 0), *px = x.p + r0 * x.ld + (col ? c : 0);
     T* ph = h + r0 * S.D + c;
@@ -414,8 +518,7 @@ __global__ void __launch_bounds__(kThreads) k_rec_step(RecShape S, Src<T> gate, 
 template <typename T, int E, int KIND>
 __global__ void __launch_bounds__(kThreads, 3) k_rec_bwd(RecShape S, int lanes_b, Src<T> gate, Src<T> x, Src<T> gh,
                                                          const float* __restrict__ h0, const float* __restrict__ ghT,
-                                                         const float* __restrict__ saved,
-                                                         const uint2* __restrict__ prefix,
+                                                         const float* __restrict__ saved, Maps prefix,
                                                          const float* __restrict__ state, T* __restrict__ ggate,
                                                          T* __restrict__ gx, float* __restrict__ gh0) {
   const int sub = threadIdx.x & (lanes_b - 1), per = kThreads / lanes_b, mine = threadIdx.x / lanes_b;
@@ -426,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_rec_bwd(RecShape S, int lanes_b
   const Edges ed = group_edges(S, g - mine % warp_groups, warp_groups, mine % warp_groups);
   const unsigned edge = ed.first | ed.none, edge_u = ed.last | ed.none;
   float u[E];
-  group_state(S, prefix, state, g, kThreads / S.lanes, c, col && g < S.groups, u);
+  group_state<MapOf<KIND>>(S, prefix, state, g, kThreads / S.lanes, c, col && g < S.groups, u);
   auto part = [&](int lo, auto plain) {
     Pack<T, E> xp[kPart], dp[kPart];
     float a[kPart][E], w[kPart][E], hp[kPart][E], s[E];
@@ -500,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_rec_bwd(RecShape S, int lanes_b
 long long groups_of(long long N) { return (N + kGroup - 1) / kGroup; }
 
 struct RecWs {
-  uint2 *prefix, *chunk;
+  Maps prefix, chunk;
   float* state;
   size_t bytes;
 };
@@ -510,8 +613,10 @@ RecWs carve(void* ws, long long N, long long D) {
   Carve c(ws);
   RecWs w;
   const long long g = groups_of(N), k = (g + kThreads / 32 - 1) / (kThreads / 32);
-  w.prefix = c.take<uint2>(g * D);
-  w.chunk = c.take<uint2>(k * D);
+  w.prefix.ac = c.take<uint2>(g * D);
+  w.chunk.ac = c.take<uint2>(k * D);
+  w.prefix.e = c.take<short>(g * D);
+  w.chunk.e = c.take<short>(k * D);
   w.state = c.take<float>(k * D);
   w.bytes = c.bytes_needed();
   return w;
@@ -570,7 +675,7 @@ void find_states(const RecShape& S, Src<T> gate, Src<T> in, const float* s0, con
   launch(k_rec_map<T, E, KIND, BWD>, dim3(S.chunks, (S.D + W - 1) / W), kThreads, 0, s, S, gate, in, s0, w.prefix,
          w.chunk);
   if (S.chunks > 1)
-    launch(k_rec_chain<BWD>, (S.D + kChainCols - 1) / kChainCols, kChainCols * kChainSegs, 0, s, w.chunk, S.chunks, S.D,
+    launch(k_rec_chain<MapOf<KIND>, BWD>, (S.D + kChainCols - 1) / kChainCols, kChainCols * kChainSegs, 0, s, w.chunk, S.chunks, S.D,
            w.state);
 }
 

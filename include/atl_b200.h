@@ -426,7 +426,7 @@ int atlb_dropout(int dtype, const void* x, const void* residual, int64_t n, doub
 
 /* Gated linear recurrence over the rows of packed windows, per column:
  *   ATLB_REC_DECAY    h_t = gate_t h_(t-1) + x_t
- *   ATLB_REC_SIGMOID  h_t = a_t h_(t-1) + (1 - a_t) x_t,  a_t = 1 / (1 + exp(-gate_t))
+ *   ATLB_REC_SIGMOID  h_t = a_t h_(t-1) + (1 - a_t) x_t,  a_t = 1 / (1 + exp(-gate_t)), zero below 2^-126
  * gate, x (N, D); b (N) the window of each row, the rows of a window contiguous (events sorted by (b, t) are; otherwise
  * each run of equal b starts from h0, and which run's hT and gh0 remain is open); rows with b outside [0, B) get h = 0
  * and no gradient.  b NULL: B equal windows of N / B rows (N a multiple of B).

@@ -106,3 +106,23 @@ def test_decay_infinite_gate_stays_in_its_column():
     h = x_b200.linear_recurrence(gate, x, kind="decay")
     assert not torch.isfinite(h[200:, 1]).any() and not torch.isfinite(h[333:, 3]).any()
     assert torch.equal(h[:, [0, 2]], clean[:, [0, 2]]) and torch.equal(h[:200, 1], clean[:200, 1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("low", [-float("inf"), -1000.0, -130.0])
+def test_closed_gates_leave_no_trace_of_a_large_state(low, dtype):
+    """A gate far below zero takes x and nothing of the state before it, of 2^120 here: exp(-130) 2^120 is below 2^-66."""
+    N, D = 700, 40
+    gate, x = torch.full((N, D), 20.0, dtype=dtype, device=DEV), randn(N, D, seed=1, dtype=dtype)
+    x[100:103] = float(2.0**120) if dtype != torch.float16 else 0.0
+    shut = torch.tensor([0, 40, 103, 330, 600], device=DEV)
+    gate[shut] = low
+    gate[100:103] = -20.0
+    gate.requires_grad_(), x.requires_grad_()
+    h0 = torch.full((1, D), 2.0**120, device=DEV, requires_grad=True)
+    h, st = x_b200.linear_recurrence(gate, x, h0=h0, return_state=True)
+    assert torch.equal(h[shut], x[shut])
+    assert h.isfinite().all() and (st.abs() < 8).all()
+    gg, gx, g0 = torch.autograd.grad(st, [gate, x, h0], torch.ones_like(st))
+    assert (gx[:600] == 0).all() and (gg[:600] == 0).all() and (g0 == 0).all() and gg.isfinite().all()
+    assert ((gx[600] - 1).abs() < 0.01).all()

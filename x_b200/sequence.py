@@ -250,7 +250,7 @@ def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, b: torch.Tensor | Non
                       h0: torch.Tensor | None = None, kind: str = "sigmoid", return_state: bool = False):
     """A state per column that runs along the rows of each window:
 
-        kind="sigmoid"  h_t = a_t h_(t-1) + (1 - a_t) x_t,  a_t = sigmoid(gate_t)
+        kind="sigmoid"  h_t = a_t h_(t-1) + (1 - a_t) x_t,  a_t = sigmoid(gate_t), zero below 2^-126
         kind="decay"    h_t = gate_t h_(t-1) + x_t          (exp(-dt / tau): decaying event traces)
 
     gate, x (N, D), one dtype; slices of a wider projection are taken as they are.  ``b`` (N,) int64 is the window of

@@ -42,7 +42,7 @@ struct RecShape {
 
 // a = 1 / (1 + exp(-z)) and 1 - a = exp(-z) a, so that neither cancels.  Below z = -87.3 a would be no normal number and
 // counts as zero, so a large state leaves no trace behind a closed gate; 1 - a is one there (exp(-z) a would be 0 inf).
-// (Holding a at exp(-87) instead left 2 % of a state of 2^120; it was 0.6 to 1.9 % faster, 1M bf16 rows of 64 both ways.)
+// (Holding a at exp(-87) let 0.02 through from a state of 2^120; it was 1.9 % faster, 1M bf16 rows of 64 both ways.)
 // FINE, for fp32 gates: expf, whose error does not grow with |z|.  For 16-bit gates the bare exponential stays below 1e-6
 // of the value for |z| < 10, far below the gates' own rounding, and is 4 % (1M rows, both ways) to 12 % (4M rows forward)
 // faster.

@@ -9,11 +9,12 @@ float32, bfloat16 and float16; sums, states and products are held in float32 and
 kernels run on the tensors' device and its current stream, allocate with torch and never synchronise, so calls can be
 captured in CUDA graphs; a backward pass only while no eager autograd graph of the same leaves lives (torch ties a
 leaf's gradient to the stream of its first graph, and the capture fails).  Results do not depend on the timing of a
-run.  There is no CPU path, and the gradients are not differentiable again.
+run.  There is no CPU path, the gradients are not differentiable again, and forward-mode derivatives are refused.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -58,6 +59,18 @@ def _rows(t):
 
 def _addr(t):
     return None if t is None else t.data_ptr()
+
+
+def _tracked(*tensors) -> bool:
+    """Does a derivative of any of the tensors (None is none) have to be tracked?  A forward-mode one as well: the autograd
+    function refuses it, as it has no forward-mode formula, where the kernel alone would drop it."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside all dual levels; asking each tensor takes a microsecond
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 # ------------------------------------------------------------------------------------------- embedding
@@ -117,7 +130,7 @@ def embedding(weight: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> to
     if idx.dtype not in _INDEX_TYPES:
         raise RuntimeError(f"x_b200.embedding: idx must be int64, int32, int16 or uint8, got {idx.dtype}")
     idx = idx.long().contiguous()
-    if weight.requires_grad and torch.is_grad_enabled():
+    if _tracked(weight):
         return _Embedding.apply(weight, idx, float(scale))
     return _embedding_fwd(weight, idx, float(scale))
 
@@ -181,7 +194,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, call=0, residual: torch.Tensor
     else:
         call = int(call) & _MASK64
     seed = int(seed) & _MASK64
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if _tracked(x, residual):
         return _Dropout.apply(x, residual, float(p), seed, call)
     return _dropout_run(x, residual, float(p), seed, call)
 
@@ -285,7 +298,7 @@ def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, b: torch.Tensor | Non
         if h0.shape != (B, D):
             raise ValueError(f"x_b200.linear_recurrence: h0 must be ({B}, {D}), got {tuple(h0.shape)}")
         h0 = h0.contiguous()
-    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+    if _tracked(gate, x, h0):
         h, state = _Recurrence.apply(gate, x, b, B, h0, code, return_state)
     else:
         h, state, _ = _recurrence_fwd(gate, x, b, B, h0, code, return_state, False)

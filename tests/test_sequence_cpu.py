@@ -2,6 +2,7 @@
 statements that the GPU tests compare with (their gradients against central differences, their random words against
 the oracle's generator)."""
 import ctypes
+import os
 
 import numpy as np
 import pytest
@@ -105,3 +106,21 @@ def test_embedding_gradient_against_differences():
         d[i] = 0.5  # linear in w: any step gives the gradient
         num = ((R.embedding(w + d, idx, 1.5)[0] - R.embedding(w - d, idx, 1.5)[0]) * g).sum()
         assert abs(num - grad[i]) < 1e-12
+
+
+def test_import_without_cuda_bindings():
+    """A torch built without CUDA has none of the private bindings; the package imports, and a call says what is missing."""
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for name in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, name)\n"
+            "import x_b200\n"
+            "try:\n"
+            "    x_b200.embedding(torch.zeros(4, 8), torch.zeros(3, dtype=torch.long))\n"
+            "except RuntimeError as e:\n"
+            "    assert 'CUDA tensor' in str(e)\n"
+            "else:\n"
+            "    raise SystemExit('no error')\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(__file__)))
+    assert r.returncode == 0, r.stderr

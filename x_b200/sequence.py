@@ -21,9 +21,10 @@ from . import _lib as L
 
 _MASK64 = 2**64 - 1
 _INDEX_TYPES = (torch.int64, torch.int32, torch.int16, torch.uint8)
-_current_device = torch._C._cuda_getDevice
-# the device's current stream as an integer: a Stream object costs several microseconds to make
-_stream = torch._C._cuda_getCurrentRawStream
+# The current device, and a device's current stream as an integer: a Stream object costs several microseconds to make.
+# The public calls stand in where a torch build lacks the bindings.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 # ------------------------------------------------------------------------------------------- arguments

@@ -34,3 +34,23 @@ def test_forward_mode_inputs_are_refused(call, grad):
         again = call(x)
     for a, b in zip((plain, again) if torch.is_tensor(plain) else plain, (again, plain) if torch.is_tensor(again) else again):
         assert torch.equal(a, b)
+
+
+def test_events_outside_the_sensor_read_zeros_and_train_nothing():
+    """Positions with fractions, on the border and outside on every side: the row of the nearest pixel, or zeros."""
+    W, H, D = 7, 5, 8
+    xy = torch.tensor([[0.0, 0.0], [6.4, 4.4], [2.6, 3.3], [7.0, 1.0], [-1.0, 2.0], [-0.4, 0.4], [3.0, -1.0], [3.0, 5.0],
+                       [6.6, 2.0], [2.0, 3.5]], device=DEV)
+    want = [0, 34, 24, -1, -1, 0, -1, -1, -1, 4 * W + 2]  # halves to even
+    xi, yi = xy.round().long().unbind(1)
+    pix = torch.where((xi >= 0) & (xi < W) & (yi >= 0) & (yi < H), yi * W + xi, -1)
+    assert pix.tolist() == want
+    table = randn(H * W, D, seed=3).requires_grad_()
+    out = x_b200.embedding(table, pix)
+    (grad,) = torch.autograd.grad(out, [table], torch.ones_like(out))
+    count = torch.zeros(H * W, device=DEV)
+    for row, n in enumerate(want):
+        assert torch.equal(out[row], table[n] if n >= 0 else torch.zeros(D, device=DEV))
+        if n >= 0:
+            count[n] += 1
+    assert torch.equal(grad, count[:, None].expand(H * W, D))

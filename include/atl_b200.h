@@ -397,20 +397,21 @@ int atlb_rng_normal2(uint64_t seed, uint64_t call, int64_t n, float* out, atlb_s
  * features per event) and whose output the objectives score.  No counterpart in the reference's ops.
  * Element types (dtype): ATLB_F32, ATLB_BF16, ATLB_F16; all arrays of one call marked `void*` have that type.  Rows
  * are contiguous; the row stride ld* (in elements, >= 0) of an input may differ from D, outputs have stride D.
- * Outputs must not overlap inputs.  Sums, states and products are fp32, and every output is rounded once.  N <= ATLB_SEQ_MAX_N, D <= ATLB_SEQ_MAX_D, row
- * strides below 2^31 in the row lookup; N * D may exceed 32 bits.
+ * Outputs must not overlap inputs.  Sums, states and products are held in 32 bits or more, and every output is rounded
+ * once.  N <= ATLB_SEQ_MAX_N, D <= ATLB_SEQ_MAX_D, row strides below 2^31 in the row lookup; N * D may exceed 32 bits.
  * ---------------------------------------------------------------------------------------------- */
 enum { ATLB_F32 = 0, ATLB_BF16 = 1, ATLB_F16 = 2 };
 #define ATLB_SEQ_MAX_D (1 << 20)
 #define ATLB_SEQ_MAX_N ((1LL << 31) - 65536) /* rows are counted in 32 bits, with room behind the last */
 
-/* Row lookup: out[n, :] = scale * weight[idx[n], :], zero where idx[n] lies outside [0, V) (as the gather reads zero
- * outside the image).  weight (V, D) with row stride ldw, idx (N), out (N, D). */
+/* Row lookup: out[n, :] = scale * weight[idx[n], :] (scale rounded to fp32), zero where idx[n] lies outside [0, V) (as
+ * the gather reads zero outside the image).  weight (V, D) with row stride ldw, idx (N), out (N, D). */
 int atlb_embedding_fwd(int dtype, const void* weight, int64_t ldw, int64_t V, int64_t D, const int64_t* idx, int64_t N,
                        double scale, void* out, atlb_stream_t stream);
 /* Its gradient: grad[v, :] = scale * sum over n with idx[n] = v of g[n, :], overwritten (rows no event reads get 0).
- * The row numbers are sorted and every run summed in the order of its events, in fp32, without atomics: the same
- * inputs give the same bits.  V < 2^31 - 1. */
+ * The row numbers are sorted and every run of equal ones summed in an order that the sizes and the row numbers fix, not
+ * one event after the other: fp32 within chunks of events, 64 bits across them, no atomics.  The same inputs give the
+ * same bits.  V < 2^31 - 1. */
 size_t atlb_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D);
 int atlb_embedding_bwd(int dtype, const void* g, int64_t ldg, const int64_t* idx, int64_t N, int64_t V, int64_t D,
                        double scale, void* grad, void* workspace, size_t workspace_bytes, atlb_stream_t stream);

@@ -52,10 +52,10 @@ __device__ __forceinline__ float drop_one(const Drop& D, unsigned word, float x)
 
 // A vector of 16 bytes is one Philox call of fp32 or two of 16-bit elements.  VECS vectors per thread, their loads
 // issued together; with four, the part of the words that a CTA shares is spread over the most calls.  fp32 runs at the
-// copy rate (2M x 48 with a residual, forward and backward: 285 us, 1.92 GB).  16-bit elements are bound by the words'
-// 32 x 32-bit products, which hold the issue port for about four cycles each: 64M bf16 elements take 57 us a pass,
-// 256 MB, 70 % of the copy rate (two vectors 59, one 60; high and low halves as two products: the same).  Element by
-// element, where a pointer is not on a 16-byte boundary, a pass takes 95 us.
+// copy rate (2M x 48 with a residual, forward and backward: 285 us, 1.92 GB).  64M bf16 elements take 57 us a pass, 256 MB,
+// 70 % of the copy rate (two vectors 59, one 60; high and low halves as two products: the same): the words' 32 x 32-bit
+// products hold the issue port for about four cycles each, 31 us, the bytes take 40, and at 57 % of the warps the two
+// overlap in part only.  Element by element, where a pointer is not on a 16-byte boundary, a pass takes 95 us.
 template <typename T, bool RES, int VECS>
 __global__ void __launch_bounds__(kThreads) k_dropout_vec(Drop D, const T* __restrict__ x, const T* __restrict__ res,
                                                           long long n, T* __restrict__ out) {
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) k_dropout(Drop D, const T* __restric
 
 template <typename T, bool RES>
 int run(const Drop& D, const T* x, const T* res, long long n, T* out, cudaStream_t s) {
-    constexpr int E = 16 / sizeof(T), VECS = 4;
+  constexpr int E = 16 / sizeof(T), VECS = 4;
   long long done = 0;
   if (aligned_to(x, 16) && aligned_to(out, 16) && (!RES || aligned_to(res, 16))) {
     const long long vecs = n / E, per = kThreads * VECS;

@@ -3,9 +3,10 @@
 //   out[n, :] = scale * W[i_n, :]                      zero where i_n lies outside [0, V)
 //   dW[v, :]  = scale * sum over n with i_n = v of g[n, :]
 //
-// The gradient sorts the row numbers first (stable, so equal rows keep the order of their events) and sums each run
-// of equal rows in fp32 in that order: no atomics, the same result every time.  Runs that cross the border of a
-// chunk leave partial sums, which a second kernel joins in order.
+// The gradient sorts the row numbers first (stable, so equal rows keep the order of their events) and sums each run of
+// equal rows in an order that N, V, D and the row numbers fix, without atomics: the same result every time.  fp32 inside
+// a chunk of the sorted events; runs that cross a chunk's border leave partial sums, which a second kernel joins in 64
+// bits.
 #include "vec.cuh"
 
 namespace atlb {
@@ -16,7 +17,9 @@ constexpr int kThreads = 256;
 // ------------------------------------------------------------------------------------------------ forward
 // A group of `lanes` threads (up to 32) takes kRowsEach rows, E neighbouring columns per thread: the rows' numbers, then
 // all their loads, then the stores.  Groups need not divide a warp: rows of 96 fp16 columns take 12 threads.  1M rows of
-// 64 bf16 columns from 307200: 42 us (175 MB, 4.2 TB/s); 4M of 96 fp16 columns from 33 rows: 172 us (800 MB, 4.7 TB/s).
+// 64 bf16 columns from 307200: 41 us (175 MB, 4.3 TB/s); 4M of 96 fp16 columns from 33 rows: 170 us (800 MB, 4.7 TB/s).
+// 63 and 79 % of the issue slots, 34 and 53 % of DRAM's peak: instructions bound it rather than bytes.  (bf16 spills one
+// pair of registers under the cap of 6 CTAs.)
 constexpr int kRowsEach = 3;  // four (5 CTAs per SM) take 45 us where three take 42, eight (4 CTAs) 80
 
 template <typename T, int E>
@@ -57,7 +60,7 @@ __global__ void __launch_bounds__(kThreads, 6) k_embed_fwd(const T* __restrict__
 // Least-significant-digit radix sort of (row, event) pairs, up to kMaxBits per pass.  A tile is 512 * ITEMS
 // neighbouring pairs; every pass counts the tiles' digits, scans the counts and places the pairs.  Tiles of 4096 pairs
 // spread the work per digit (a place per warp and digit to clear and to sum) over more pairs: lookup and gradient of 1M
-// events 190 us against 195 with 2048.  Below 64 tiles of that size the GPU would idle, and tiles of 2048 are taken.
+// events 152 us on the device against 160 with 2048.  Below 64 tiles of that size the GPU would idle, and tiles of 2048 are taken.
 // 1M pairs take 20 us a placement, bound by the latency of its steps (28 % of issue slots, 5 % of DRAM).
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
@@ -347,8 +350,9 @@ SortPlan sort_plan(long long N, long long V) {
 // A group of `lanes` threads walks the L sorted pairs of one chunk, keeping E columns per thread in fp32, and
 // writes a gradient row when its run ends inside the chunk.  A run that came in from the chunk before leaves its
 // sum in part[chunk][0], one that goes on into the next chunk in part[chunk][1] (in [0] if it does both).  Bound by its
-// scattered row reads: 1M rows of 64 bf16 columns 40 us (137 MB from DRAM, 3.8 TB/s), 4M of 96 fp16 columns 171 us
-// (995 MB, 5.8 TB/s; rows of 192 bytes fetch parts of lines that others need later).
+// scattered row reads: 1M rows of 64 bf16 columns 42 us (149 MB of DRAM traffic, 3.5 TB/s), 4M of 96 fp16 columns 161 us
+// (995 MB, 6.2 TB/s; rows of 192 bytes fetch parts of lines that others need later).  The order of a chunk's sum: fours of
+// neighbouring events that share their row, (a + b) + (c + d), one event at a time where a four holds a border.
 constexpr int kAhead = 4;  // rows in flight per thread, at 3 CTAs per SM: 4 CTAs with spilled registers took 47 us
 
 template <typename T, int E>
@@ -430,7 +434,8 @@ __global__ void __launch_bounds__(kThreads, 3) k_embed_sum(const T* __restrict__
 // The chunk in which a run over several chunks begins joins its partial sums.  A CTA looks after 32 chunks: a warp each
 // for the runs that go on over fewer than 32 more chunks, in order; then, for a longer one, all its threads, 64 rows of
 // them over 16 columns: each takes every 64th partial sum, and these are added in order.  The few sums of sums are taken
-// in 64 bits, which costs nothing here and keeps long runs at the error of their chunks.
+// in 64 bits, which keeps long runs at the error of their chunks (1M events, lookup and gradient: 152 us on the device,
+// 151 with fp32).
 constexpr int kJoinThreads = 1024, kLongCols = 16, kLongRows = kJoinThreads / kLongCols;
 
 template <typename T>
@@ -541,7 +546,7 @@ int embedding_fwd(int dtype, const void* W, long long ldw, long long V, long lon
     const int E1 = wide ? E : 1;
     const long long per = kThreads / lanes * kRowsEach;
     const unsigned slabs = (unsigned)((D + lanes * E1 - 1) / (lanes * E1));
-        const dim3 grid((unsigned)((N + per - 1) / per), slabs);
+    const dim3 grid((unsigned)((N + per - 1) / per), slabs);
     auto go = [&](auto el) {
       launch(k_embed_fwd<T, decltype(el)::value>, grid, kThreads, 0, s, (const T*)W, (int)ldw, (int)V, (int)D, idx, (int)N,
              (float)scale, lanes, (T*)out);

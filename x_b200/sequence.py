@@ -5,7 +5,7 @@ The objectives score a motion; a model that produces it from events needs, per e
 events (:func:`linear_recurrence`).  All three work on the layout of the other ops of this package: one row per event,
 windows packed one behind the other and sorted by (b, t), ``b`` (N,) int64.  The reference's ops have no counterpart.
 
-float32, bfloat16 and float16; sums, states and products are held in float32 and every output is rounded once.  The
+float32, bfloat16 and float16; sums, states and products are held in float32 or more and every output is rounded once.  The
 kernels run on the tensors' device and its current stream, allocate with torch and never synchronise, so calls can be
 captured in CUDA graphs; a backward pass only while no eager autograd graph of the same leaves lives (torch ties a
 leaf's gradient to the stream of its first graph, and the capture fails).  Results do not depend on the timing of a
@@ -122,8 +122,9 @@ def embedding(weight: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> to
 
     weight (V, D) float32, bfloat16 or float16; idx integers of any shape.  An index outside [0, V) reads a row of
     zeros and gives no gradient, as :func:`x_b200.gather` does outside the image: events that left the sensor and
-    padding (-1) need no mask.  The gradient of ``weight`` is summed over the events of each row in their order, in
-    float32 and without atomics; rows that no event reads get zeros."""
+    padding (-1) need no mask.  The gradient of ``weight`` is summed over the events of each row without atomics, in an
+    order that depends on the sizes and ``idx`` alone (float32 within chunks of events, float64 across them); rows that
+    no event reads get zeros."""
     _device("embedding", "weight", weight, idx=idx)
     if weight.dim() != 2:
         raise ValueError(f"x_b200.embedding: weight must be (V, D), got {tuple(weight.shape)}")

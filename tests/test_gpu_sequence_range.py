@@ -98,6 +98,26 @@ def test_decay_gates_of_zero_and_at_the_ends_of_fp32(D):
     compare("decay", gate, x, None, 1, h0, gh, randn(1, D, seed=5))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("low", [0.0, 2.0**-14, 2.0**-3])
+def test_decay_short_memories(low, dtype):
+    """Gates that are zero or small in most rows, one among them or all of a group, and rows of ones around them: what
+    passes is lost or kept to the bit.  x and gradients are whole numbers; the small gates are powers of two."""
+    N, D = 1800, 40
+    gate = torch.ones(N, D, device=DEV)
+    pick = torch.rand(N, D, generator=gen(1), device=DEV)
+    gate[600:1200] = torch.where(pick[600:1200] < 0.3, low, 1.0)
+    gate[1300:1340] = low
+    gate[::50, ::3] = low
+    gate = gate.to(dtype).requires_grad_()
+    x = torch.randint(-3, 4, (N, D), generator=gen(2), device=DEV).to(dtype).requires_grad_()
+    gh = torch.randint(-3, 4, (N, D), generator=gen(3), device=DEV).to(dtype)
+    h0, ghT = randn(1, D, seed=4).requires_grad_(), randn(1, D, seed=5)
+    got, r = compare("decay", gate, x, None, 1, h0, gh, ghT)
+    if low == 0.0:  # nothing but whole numbers behind a zero
+        assert (got[0][1340:1350].float() == got[0][1340:1350].float().round()).all() and torch.equal(got[0][1339], x[1339])
+
+
 def test_decay_infinite_gate_stays_in_its_column():
     N, D = 900, 4
     gate, x = torch.full((N, D), 0.5, device=DEV), randn(N, D, seed=1)

@@ -87,8 +87,10 @@ __device__ __forceinline__ float apply(const Map& m, float s) { return m.cut ? m
 __device__ __forceinline__ Map then(const Map& a, const Map& b) { return Map{a.A * b.A, apply(b, a.C), a.cut || b.cut}; }
 
 // Decay: gates of any size.  A product over a chunk may leave fp32's range where no state does (130 gates of 2 and 130 of
-// 1/2 behind a state of 0.01), so A = m 2^e with |m| in [1, 2), or m zero, infinite or NaN.  Device time of 1M bf16 rows of
-// 64 columns, both ways: 364 us, where plain fp32 products took 349; 100k fp32 rows of 32: 48 and 45.
+// 1/2 behind a state of 0.01), so A = m 2^e with |m| in [1, 2), or m = e = 0 for zero;
+// where a gate is infinite or a NaN, so is C, and m says nothing.  Device time of 1M bf16 rows of
+// 64 columns, both ways: 367 us, where plain fp32 products took 348 (with 1 % of zero gates 353 for 347 unpacked); 100k
+// fp32 rows of 32: 48 and 44.
 struct WideMap {
   float m, C;
   int e;
@@ -117,6 +119,54 @@ __device__ __forceinline__ void split(float v, float* m, int* e) {
   const bool plain = x != 255 && v != 0.f;
   *m = plain ? __uint_as_float((b & 0x807fffffu) | 0x3f800000u) : v;
   *e = plain ? x - (small ? 191 : 127) : 0;
+}
+// A 2^x times the gates of four rows, per column; |A| in [1, 2).  Their product is a normal number on the whole way where
+// none is above 2^8 and the end is at least 2^-100.  A gate of zero takes the exponent far below any other's sum and leaves
+// A as it was; where gates are too large or too small all the same, each one's exponent is taken apart.
+constexpr int kZeroExp = -(1 << 20);
+template <typename T, int E>
+__device__ __forceinline__ void times(const Pack<T, E> (&gate)[4], float (&A)[E], int (&x)[E]) {
+  float p[E];
+  bool plain = true;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float a = to_f32(gate[0].v[e]), b = to_f32(gate[1].v[e]), c = to_f32(gate[2].v[e]), d = to_f32(gate[3].v[e]);
+    p[e] = A[e] * a * b * c * d;
+    plain = plain && fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d))) <= 0x1p8f && fabsf(p[e]) >= 0x1p-100f;
+  }
+  if (!plain) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float top = 0.f;
+      bool zero = false;
+      p[e] = A[e];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = to_f32(gate[j].v[e]);
+        zero = zero || a == 0.f;
+        p[e] *= a == 0.f ? 1.f : a;
+        top = fmaxf(top, fabsf(a));
+      }
+      if (zero) x[e] += kZeroExp;
+      if (!(top <= 0x1p8f && fabsf(p[e]) >= 0x1p-100f)) {
+        p[e] = A[e];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float m;
+          int k;
+          split(to_f32(gate[j].v[e]), &m, &k);
+          if (m != 0.f) p[e] *= m;
+          x[e] += k;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const unsigned b = __float_as_uint(p[e]);
+    x[e] += (int)(b >> 23 & 255) - 127;
+    A[e] = __uint_as_float((b & 0x807fffffu) | 0x3f800000u);
+  }
 }
 
 // Arrays of maps: A and C as 64 bits (a cut stands in the place of A, as a NaN that arithmetic does not make), or m and C
@@ -242,9 +292,13 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
   const bool col = c < S.D;
   const Edges ed = group_edges(S, g - mine % warp_groups, warp_groups, mine % warp_groups);
   const unsigned edge = (BWD ? ed.last : ed.first) | ed.none;
-  float A[E], s[E], hi = 1.f, lo = 1.f;  // hi, lo: the largest and the smallest magnitude that A went through
+  float A[E], s[E];
+  int x[kWide ? E : 1];  // A's exponents, where they are kept apart
 #pragma unroll
-  for (int e = 0; e < E; ++e) { A[e] = 1.f; s[e] = 0.f; }
+  for (int e = 0; e < E; ++e) {
+    A[e] = 1.f, s[e] = 0.f;
+    if (kWide) x[e] = 0;
+  }
   auto rows = [&](auto plain) {
     // rows are stepped through by pointer: a product with the stride per row costs as much as four additions.  Threads
     // behind the last column read the first and are not heard.
@@ -262,6 +316,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
         pg += dg;
         pi += di;
       }
+      if constexpr (kWide) times(gp, A, x);
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int r = BWD ? kGroup - 1 - q - j : q + j;
@@ -274,11 +329,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
           float a, w, v;
           row_terms<KIND>(gp[j].v[e], ip[j].v[e], &a, &w, &v);
           s[e] = BWD ? a * (to_f32(ip[j].v[e]) + s[e]) : fmaf(a, s[e], v);
-          A[e] *= a;
-          if (kWide) {
-            hi = fmaxf(hi, fabsf(A[e]));
-            lo = fminf(lo, fabsf(A[e]));
-          }
+          if (!kWide) A[e] *= a;
         }
       }
     }
@@ -289,27 +340,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
     rows(std::true_type());
   // joined along the walk, per column: kSeg groups by one thread, then the segments, then the groups again
   const int at = BWD ? per - 1 - mine : mine, segs = (per + kSeg - 1) / kSeg;
-  // A product that left the normal numbers, or came near: the gates once more, their exponents summed apart.  Without a
-  // border the group's rows all exist.
-  const bool far = kWide && edge == 0 && col && !(hi <= 0x1p100f && lo >= 0x1p-100f);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if constexpr (kWide) {
-      WideMap m{A[e], s[e], 0, edge != 0};
-      if (far) {
-        m.m = 1.f;
-#pragma unroll 1
-        for (int r = 0; r < kGroup; ++r) {
-          WideMap row{0.f, 0.f, 0, false};
-          split(to_f32(gate.p[(r0 + r) * gate.ld + c + e]), &row.m, &row.e);
-          m.m *= row.m;
-          m.e += row.e;
-        }
-      }
-      int x;
-      split(m.m, &m.m, &x);
-      m.e += x;
-      sm.put(at * W + sub * E + e, m);
+      const bool zero = x[e] < kZeroExp / 2;
+      sm.put(at * W + sub * E + e, WideMap{zero ? 0.f : A[e], s[e], zero ? 0 : x[e], edge != 0});
     } else {
       sm.put(at * W + sub * E + e, Map{A[e], s[e], edge != 0});
     }
@@ -318,10 +353,15 @@ __global__ void __launch_bounds__(kThreads, 4) k_rec_map(RecShape S, Src<T> gate
   for (int i = threadIdx.x; i < segs * W; i += kThreads) {
     const int x = i % W, k0 = i / W * kSeg;
     M m = M::identity();
-    for (int k = k0; k < k0 + kSeg && k < per; ++k) {
-      const M next = map_at<M>(sm, k * W + x);
-      sm.put(k * W + x, m);
-      m = then(m, next);
+    for (int k = k0; k < k0 + kSeg && k < per; k += 4) {  // per is a multiple of eight; four loads on the way at once
+      M next[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) next[j] = map_at<M>(sm, (k + j) * W + x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sm.put((k + j) * W + x, m);
+        m = then(m, next[j]);
+      }
     }
     seg.put(i, m);
   }

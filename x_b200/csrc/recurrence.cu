@@ -12,8 +12,8 @@
 // chunk of groups (k_rec_map); the states between the chunks (k_rec_chain); the rows replayed from the true state of
 // their group (k_rec_fwd, k_rec_bwd).  Inputs are read twice and nothing waits for another CTA: a single pass, with
 // tiles in shared memory that post their maps to one another, reads them once but measured 647 us where this form took
-// 376 (forward and backward, 1M rows of 64 bf16 columns; 382 now), the waits and the link costing more than the bytes.
-// What bounds it is memory: 4M rows of 64 fp16 columns forward move 2.6 GB in 493 us (5.3 TB/s, 82 % of the copy rate),
+// 376 (forward and backward, 1M rows of 64 bf16 columns; 378 now), the waits and the link costing more than the bytes.
+// What bounds it is memory: 4M rows of 64 fp16 columns forward move 2.6 GB in 496 us (5.3 TB/s, 82 % of the copy rate),
 // where one reading would be 1.5 GB.  Measured against 374 / 240 / 483 us (1M rows of 64 both ways; 16 windows of 2048
 // rows of 1024; 4M rows forward): 16 bytes per thread 429 / 263 / 535, 8 rows in flight 404 / 264 / 515, rows through a
 // ring in shared memory 399 / 241 / 549, CTAs of 128 threads 383 / 229 / 505, packed fp32 arithmetic 371 / 232 / 485,
@@ -273,8 +273,8 @@ struct Src {
 // ------------------------------------------------------------------------------------------------ maps of the groups
 // Threads `lanes` wide on a row, E neighbouring columns each; the CTA's groups are one chunk.  BWD walks from the last
 // row to the first: in = dL/dh, and the state is u.  prefix: the map from the chunk's entry to the group's; chunk: the
-// whole chunk's map.  1M rows of 64 bf16 columns: 66 us forward, 62 backward, 280 MB (4.2 and 4.5 TB/s); 4M rows 201 us
-// (5.4 TB/s).
+// whole chunk's map.  1M rows of 64 bf16 columns: 65 us forward, 61 backward, 277 MB (4.3 and 4.5 TB/s); 4M rows 198 us
+// (5.5 TB/s).
 constexpr int kAhead = 4;  // rows in flight per thread
 
 template <typename T, int E, int KIND, bool BWD>
@@ -465,10 +465,10 @@ __device__ __forceinline__ void group_state(const RecShape& S, const Maps& prefi
 }
 
 // ------------------------------------------------------------------------------------------------ replay, forward
-// 1M rows of 64 bf16 columns: 75 us, 400 MB of DRAM traffic with the kept states (5.3 TB/s); 4M fp16 rows without them
+// 1M rows of 64 bf16 columns: 73 us, 400 MB of DRAM traffic with the kept states (5.5 TB/s); 4M fp16 rows without them
 // 235 us (6.7 TB/s).  Under the cap of 5 CTAs (48 registers) four bf16 columns spill 68 bytes a thread.  A cap of 4 has no
-// spills: 367 and 228 us on the device for 1M rows of 64 and 32k of 1024, both ways, where 5 take 368 and 233, but 470
-// for 4M fp16 rows forward, where 5 take 463.
+// spills: 362 and 225 us on the device for 1M rows of 64 and 32k of 1024, both ways, where 5 take 365 and 230, but 466
+// for 4M fp16 rows forward, where 5 take 459.
 template <typename T, int E, int KIND>
 __global__ void __launch_bounds__(kThreads, 5) k_rec_fwd(RecShape S, Src<T> gate, Src<T> x, const float* __restrict__ h0,
                                                       Maps prefix, const float* __restrict__ state, T* __restrict__ h,
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kThreads) k_rec_step(RecShape S, Src<T> gate, 
 // lanes_b threads on a row, E columns each (4 bytes), a group per `lanes_b` threads.  Each part of the group, the last
 // one first: its rows in registers, the states forward from the one the forward pass kept, then u backward.  The states
 // are found again in fp32 rather than read from h, which was rounded: h - x would lose what the gate's gradient needs.
-// 1M rows of 64 bf16 columns: 143 us, 660 MB (4.6 TB/s).  (16-bit sigmoid rows spill 12 to 20 bytes a thread under the cap.)
+// 1M rows of 64 bf16 columns: 145 us, 660 MB (4.6 TB/s).  (16-bit sigmoid rows spill 12 to 20 bytes a thread under the cap.)
 template <typename T, int E, int KIND>
 __global__ void __launch_bounds__(kThreads, 3) k_rec_bwd(RecShape S, int lanes_b, Src<T> gate, Src<T> x, Src<T> gh,
                                                          const float* __restrict__ h0, const float* __restrict__ ghT,
